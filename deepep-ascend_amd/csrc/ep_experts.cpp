@@ -1,0 +1,253 @@
+// Host side of the experts' computation (ep_experts.hip): argument contracts of its C entries and the launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "ep_expert_args.h"
+#include "ep_host.h"
+
+namespace {
+
+struct ExpertKernels {
+    hipModule_t module = nullptr;
+    int device = -1;
+    hipFunction_t bf16, fp8, transposed, weights[2], swiglu[2], swiglu_grad;
+};
+ExpertKernels g_k;
+std::mutex g_mutex;
+
+// (contracts are checked before: they need no GPU)
+const ExpertKernels& kernels() {
+    ep_load_expert_kernels(nullptr);
+    int cur = -1;
+    HIP_CHECK(hipGetDevice(&cur));
+    EP_HOST_ASSERT(cur == g_k.device and "the kernels were loaded on another device");
+    return g_k;
+}
+
+template <class A>
+void launch(hipFunction_t fn, int64_t grid, unsigned block, void* stream, A& args) {
+    EP_HOST_ASSERT(grid > 0 and grid * block <= UINT32_MAX);
+    void* params[] = {&args};
+    HIP_CHECK(hipModuleLaunchKernel(fn, (unsigned)grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, params, nullptr));
+}
+
+// Rows whose channels are contiguous and start on 16 bytes.
+bool row_major(const ep_tensor_t& t) {
+    if (not present(t) or t.ndim != 2 or t.size[0] < 0 or t.size[1] <= 0) return false;
+    const int64_t elem = elem_size(t.dtype);
+    if (t.size[1] != 1 and t.stride[1] != 1) return false;
+    if (t.size[0] > 1 and (t.stride[0] < t.size[1] or t.stride[0] * elem % 16 != 0)) return false;
+    return ((uintptr_t)t.data & 15) == 0;
+}
+int64_t row_stride(const ep_tensor_t& t) { return t.size[0] > 1 ? t.stride[0] : (t.size[1] + 15) / 16 * 16; }
+
+// Bytes of a tile's rows are counted in 31 bits.
+constexpr int64_t kMaxRowBytes = 4 << 20;
+bool addressable(const ep_tensor_t& t) { return row_stride(t) * elem_size(t.dtype) <= kMaxRowBytes; }
+
+EpExpertLayout layout_of(const ep_tensor_t& psum, int num_experts, int alignment, int zero_rows, int64_t rows) {
+    EP_HOST_ASSERT(num_experts > 0 and alignment > 0);
+    EP_HOST_ASSERT(zero_rows >= EP_ZERO_NONE and zero_rows <= EP_ZERO_ALL);
+    EP_HOST_ASSERT(rows + alignment <= INT32_MAX);
+    if (present(psum)) {
+        EP_HOST_ASSERT(psum.ndim == 1 and psum.dtype == EP_DTYPE_I32 and contiguous(psum));
+        EP_HOST_ASSERT(psum.size[0] == num_experts);
+    } else {
+        EP_HOST_ASSERT(num_experts == 1);
+    }
+    EpExpertLayout l{};
+    l.psum = (const int*)psum.data;
+    l.num_experts = num_experts;
+    l.alignment = alignment;
+    l.num_rows = (int)rows;
+    l.zero_rows = zero_rows;
+    return l;
+}
+
+// Row tiles of all experts are at most this many: every expert with rows begins a tile of its own.
+int64_t row_tiles_bound(const EpExpertLayout& l, int tile) {
+    return l.num_rows / tile + std::min<int64_t>(l.num_experts, l.num_rows);
+}
+
+constexpr int kTile = 128;
+
+}  // namespace
+
+void ep_load_expert_kernels(const char* dir) {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (g_k.module != nullptr) return;
+    const std::string path = ep_code_object_path(dir, "ep_experts.hsaco");
+    int ndev = 0;
+    HIP_CHECK(hipGetDeviceCount(&ndev));
+    if (ndev <= 0) throw EpError{"no HIP device visible: the EP kernels only run on a gfx950 GPU"};
+    HIP_CHECK(hipGetDevice(&g_k.device));
+    hipModule_t m;
+    HIP_CHECK(hipModuleLoad(&m, path.c_str()));
+    auto get = [&](hipFunction_t& fn, const char* name) { HIP_CHECK(hipModuleGetFunction(&fn, m, name)); };
+    get(g_k.bf16, "ep_grouped_bf16");
+    get(g_k.fp8, "ep_grouped_fp8");
+    get(g_k.transposed, "ep_grouped_transposed_bf16");
+    get(g_k.weights[0], "ep_grouped_weights_bf16");
+    get(g_k.weights[1], "ep_grouped_weights_f32");
+    get(g_k.swiglu[0], "ep_swiglu_bf16");
+    get(g_k.swiglu[1], "ep_swiglu_fp8");
+    get(g_k.swiglu_grad, "ep_swiglu_gradients");
+    g_k.module = m;
+}
+
+extern "C" {
+
+int ep_grouped_linear(const ep_grouped_linear_args_t* args) {
+    return guarded([&] {
+        EP_HOST_ASSERT(args != nullptr);
+        const ep_tensor_t &x = args->x, &w = args->weight, &out = args->out;
+        EP_HOST_ASSERT(row_major(x) and addressable(x));
+        EP_HOST_ASSERT(row_major(w) and addressable(w) and w.dtype == x.dtype);
+        const bool fp8 = x.dtype == EP_DTYPE_FP8_E4M3, transposed = args->transpose_weight != 0;
+        EP_HOST_ASSERT(fp8 or x.dtype == EP_DTYPE_BF16);
+        EP_HOST_ASSERT(not (fp8 and transposed));
+        const int64_t rows = x.size[0], depth = x.size[1], columns = w.size[transposed ? 1 : 0];
+        EP_HOST_ASSERT(w.size[transposed ? 0 : 1] == depth);
+        EP_HOST_ASSERT(depth % (fp8 ? 16 : 8) == 0 and columns > 0 and columns % 8 == 0);
+        EP_HOST_ASSERT(depth <= INT32_MAX / 2 and columns <= INT32_MAX / 2);
+        EP_HOST_ASSERT(args->num_experts == 1 or (args->weight_expert_stride >= 0 and args->weight_expert_stride * elem_size(w.dtype) % 16 == 0));
+        EP_HOST_ASSERT(row_major(out) and out.dtype == EP_DTYPE_BF16);
+        EP_HOST_ASSERT(out.size[0] == rows and out.size[1] == columns);
+        EpGemmArgs g{};
+        g.layout = layout_of(args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment, args->zero_rows, rows);
+        g.rows = (const char*)x.data;
+        g.columns = (const char*)w.data;
+        g.rows_ld = row_stride(x) * elem_size(x.dtype);
+        g.columns_ld = row_stride(w) * elem_size(w.dtype);
+        g.columns_expert = args->weight_expert_stride * elem_size(w.dtype);
+        g.out = (char*)out.data;
+        g.out_ld = row_stride(out);
+        g.depth = (int)depth;
+        g.num_columns = (int)columns;
+        EP_HOST_ASSERT(fp8 == present(args->x_sf) and fp8 == present(args->weight_sf));
+        if (fp8) {
+            const ep_tensor_t &sf = args->x_sf, &wsf = args->weight_sf;
+            EP_HOST_ASSERT(depth <= EP_EXPERT_MAX_DEPTH_FP8);
+            EP_HOST_ASSERT(sf.ndim == 2 and sf.dtype == EP_DTYPE_F32 and sf.size[0] == rows and sf.size[1] == ceil_div(depth, 128));
+            EP_HOST_ASSERT(sf.stride[0] >= 0 and sf.stride[1] >= 0 and (rows <= 1 or sf.stride[0] * 4 <= kMaxRowBytes));
+            EP_HOST_ASSERT(wsf.ndim == 2 and wsf.dtype == EP_DTYPE_F32);
+            EP_HOST_ASSERT(wsf.size[0] == ceil_div(columns, 128) and wsf.size[1] == ceil_div(depth, 128));
+            g.rows_sf = (const float*)sf.data;
+            g.columns_sf = (const float*)wsf.data;
+            g.rows_sf_row = rows > 1 ? sf.stride[0] : 1;
+            g.rows_sf_col = sf.stride[1];
+            g.columns_sf_row = wsf.stride[0];
+            g.columns_sf_col = wsf.stride[1];
+            g.columns_sf_expert = args->weight_sf_expert_stride;
+        }
+        if (rows == 0) return;
+        g.column_tiles = (int)ceil_div(columns, kTile);
+        const ExpertKernels& k = kernels();
+        launch(fp8 ? k.fp8 : transposed ? k.transposed : k.bf16, align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256,
+               args->stream, g);
+    });
+}
+
+int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
+    return guarded([&] {
+        EP_HOST_ASSERT(args != nullptr);
+        const ep_tensor_t &grad = args->grad, &x = args->x, &out = args->out;
+        EP_HOST_ASSERT(row_major(grad) and grad.dtype == EP_DTYPE_BF16 and addressable(grad));
+        EP_HOST_ASSERT(row_major(x) and x.dtype == EP_DTYPE_BF16 and addressable(x));
+        EP_HOST_ASSERT(x.size[0] == grad.size[0] and x.size[1] % 8 == 0 and grad.size[1] % 8 == 0);
+        const bool f32 = out.dtype == EP_DTYPE_F32;
+        EP_HOST_ASSERT(row_major(out) and (f32 or out.dtype == EP_DTYPE_BF16));
+        EP_HOST_ASSERT(out.size[0] == grad.size[1] and out.size[1] == x.size[1]);
+        EP_HOST_ASSERT(f32 or args->accumulate == 0);
+        EP_HOST_ASSERT(args->num_experts == 1 or
+                       (args->out_expert_stride >= out.size[0] * row_stride(out) and args->out_expert_stride * elem_size(out.dtype) % 16 == 0));
+        EpGemmArgs g{};
+        g.layout = layout_of(args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment, 0, x.size[0]);
+        g.rows = (const char*)grad.data;
+        g.columns = (const char*)x.data;
+        g.rows_ld = row_stride(grad) * 2;
+        g.columns_ld = row_stride(x) * 2;
+        g.out = (char*)out.data;
+        g.out_ld = row_stride(out);
+        g.out_expert = args->out_expert_stride;
+        g.num_columns = (int)x.size[1];
+        g.num_out_rows = (int)grad.size[1];
+        g.column_tiles = (int)ceil_div(g.num_columns, kTile);
+        g.row_tiles = (int)ceil_div(g.num_out_rows, kTile);
+        g.accumulate = args->accumulate != 0;
+        const int64_t tiles = (int64_t)g.layout.num_experts * g.row_tiles;
+        EP_HOST_ASSERT(tiles <= INT32_MAX / std::max(1, g.column_tiles));
+        launch(kernels().weights[f32 ? 1 : 0], align_up(tiles * g.column_tiles, 8), 256, args->stream, g);
+    });
+}
+
+static EpSwigluArgs swiglu_args(const ep_tensor_t& h, const ep_tensor_t& weights, const ep_tensor_t& psum, int num_experts, int alignment,
+                                int zero_rows) {
+    EP_HOST_ASSERT(row_major(h) and h.dtype == EP_DTYPE_BF16 and h.size[1] % 16 == 0 and h.size[1] <= INT32_MAX / 2);
+    EpSwigluArgs s{};
+    s.layout = layout_of(psum, num_experts, alignment, zero_rows, h.size[0]);
+    s.h = (const char*)h.data;
+    s.h_ld = row_stride(h);
+    s.channels = (int)(h.size[1] / 2);
+    if (present(weights)) {
+        EP_HOST_ASSERT(weights.ndim == 1 and weights.dtype == EP_DTYPE_F32 and weights.size[0] == h.size[0] and contiguous(weights));
+        s.weights = (const float*)weights.data;
+    }
+    s.num_parts = (int)ceil_div(s.channels, 512);
+    return s;
+}
+
+int ep_swiglu(const ep_swiglu_args_t* args) {
+    return guarded([&] {
+        EP_HOST_ASSERT(args != nullptr);
+        const ep_tensor_t &out = args->out, &sf = args->out_sf;
+        EpSwigluArgs s = swiglu_args(args->h, args->weights, args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment,
+                                     args->zero_rows);
+        const bool fp8 = out.dtype == EP_DTYPE_FP8_E4M3;
+        EP_HOST_ASSERT(present(out) and out.ndim == 2 and (fp8 or out.dtype == EP_DTYPE_BF16));
+        EP_HOST_ASSERT(out.size[0] == args->h.size[0] and out.size[1] == s.channels);
+        EP_HOST_ASSERT(out.stride[1] == 1 and (out.size[0] <= 1 or (out.stride[0] >= out.size[1] and out.stride[0] % 8 == 0)));
+        EP_HOST_ASSERT(((uintptr_t)out.data & (fp8 ? 7 : 15)) == 0);
+        s.out = (char*)out.data;
+        s.out_ld = row_stride(out);
+        EP_HOST_ASSERT(fp8 == present(sf));
+        if (fp8) {
+            EP_HOST_ASSERT(sf.ndim == 2 and sf.dtype == EP_DTYPE_F32 and sf.size[0] == out.size[0] and sf.size[1] == ceil_div(s.channels, 128));
+            s.sf = (float*)sf.data;
+            s.sf_row = sf.stride[0];
+            s.sf_col = sf.stride[1];
+        }
+        if (s.layout.num_rows == 0) return;
+        s.parts_per_task = s.num_parts;
+        const int64_t tasks = (int64_t)s.layout.num_rows * ceil_div(s.num_parts, s.parts_per_task);
+        launch(kernels().swiglu[fp8 ? 1 : 0], ceil_div(tasks, 4), 256, args->stream, s);
+    });
+}
+
+int ep_swiglu_grad(const ep_swiglu_grad_args_t* args) {
+    return guarded([&] {
+        EP_HOST_ASSERT(args != nullptr);
+        const ep_tensor_t &grad = args->grad, &grad_h = args->grad_h, &grad_weights = args->grad_weights;
+        EpSwigluArgs s = swiglu_args(args->h, args->weights, args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment,
+                                     args->zero_rows);
+        EP_HOST_ASSERT(row_major(grad) and grad.dtype == EP_DTYPE_BF16);
+        EP_HOST_ASSERT(grad.size[0] == args->h.size[0] and grad.size[1] == s.channels);
+        EP_HOST_ASSERT(row_major(grad_h) and grad_h.dtype == EP_DTYPE_BF16);
+        EP_HOST_ASSERT(grad_h.size[0] == args->h.size[0] and grad_h.size[1] == args->h.size[1]);
+        s.grad_out = (const char*)grad.data;
+        s.grad_out_ld = row_stride(grad);
+        s.grad_h = (char*)grad_h.data;
+        s.grad_h_ld = row_stride(grad_h);
+        if (present(grad_weights)) {
+            EP_HOST_ASSERT(grad_weights.ndim == 1 and grad_weights.dtype == EP_DTYPE_F32 and grad_weights.size[0] == grad.size[0]);
+            EP_HOST_ASSERT(contiguous(grad_weights));
+            s.grad_weights = (float*)grad_weights.data;
+        }
+        if (s.layout.num_rows == 0) return;
+        launch(kernels().swiglu_grad, ceil_div(s.layout.num_rows, 4), 256, args->stream, s);
+    });
+}
+
+}  // extern "C"

@@ -17,9 +17,9 @@
 #include <string>
 #include <vector>
 
-#include "../../include/deep_ep_hip.h"
 #include "ep_args.h"
 #include "ep_fp8.h"
+#include "ep_host.h"
 
 void ep_static_scratch_init();      // looks up this device's copy of the static scratch (end of this file)
 
@@ -30,52 +30,6 @@ constexpr int kUbAlign = 32;                   // reference: common/compiled.hpp
 constexpr int64_t kWorkspaceBytes = 16 * 1024 * 1024;
 
 thread_local std::string g_err;
-
-struct EpError {
-    std::string msg;
-};
-
-std::string format(const char* fmt, ...) {
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    return buf;
-}
-
-#define EP_HOST_ASSERT(cond)                                                                        \
-    do {                                                                                            \
-        if (!(cond)) throw EpError{format("Assertion exception (%s:%d): %s", __FILE_NAME__, __LINE__, #cond)}; \
-    } while (0)
-
-#define EP_HOST_UNREACHABLE(reason) \
-    throw EpError { format("Assertion exception (%s:%d): %s", __FILE_NAME__, __LINE__, reason) }
-
-#define HIP_CHECK(cmd)                                                                              \
-    do {                                                                                            \
-        const hipError_t e_ = (cmd);                                                                \
-        if (e_ != hipSuccess)                                                                       \
-            throw EpError{format("HIP runtime exception (%s:%d): Error code: %d, detail: %s", __FILE_NAME__, \
-                                 __LINE__, (int)e_, hipGetErrorString(e_))};                        \
-    } while (0)
-
-template <class F>
-int guarded(F&& f) {
-    try {
-        f();
-        return 0;
-    } catch (const EpError& e) {
-        g_err = e.msg;
-        return 1;
-    } catch (const std::exception& e) {
-        g_err = e.what();
-        return 1;
-    }
-}
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // ---- token layout (reference: layout/ep/token.hpp:9-83) -------------------------------------
 int64_t token_bytes(int hidden_bytes, int sf_bytes, int topk, bool with_metadata) {
@@ -169,21 +123,10 @@ constexpr int kPacedRowBlocks = 8192;
 std::atomic<int> g_recount_limit{-1};     // blocks x top-k up to which one partition's slot assignment counts all ids itself; negative: recount_pays
 std::atomic<int> g_fold_max_blocks{256};    // up to this many layout workgroups the slot assignment sums the block counts itself
 
-std::string library_dir() {
-    Dl_info info;
-    if (dladdr((void*)&library_dir, &info) == 0 || info.dli_fname == nullptr) return ".";
-    std::string p = info.dli_fname;
-    const auto pos = p.find_last_of('/');
-    return pos == std::string::npos ? "." : p.substr(0, pos);
-}
-
 void load_kernels(const char* dir) {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (g_k.module != nullptr) return;
-    const std::string path = (dir != nullptr ? std::string(dir) : library_dir()) + "/ep_kernels.hsaco";
-    FILE* f = fopen(path.c_str(), "rb");
-    if (f == nullptr) throw EpError{"cannot open the gfx950 code object " + path + " (build it first)"};
-    fclose(f);
+    const std::string path = ep_code_object_path(dir, "ep_kernels.hsaco");
     int ndev = 0;
     HIP_CHECK(hipGetDeviceCount(&ndev));
     if (ndev <= 0) throw EpError{"no HIP device visible: the EP kernels only run on a gfx950 GPU"};
@@ -269,29 +212,25 @@ void launch(hipFunction_t fn, unsigned grid, unsigned block, unsigned smem, void
     HIP_CHECK(hipModuleLaunchKernel(fn, grid, 1, 1, block, 1, 1, smem, (hipStream_t)stream, params, nullptr));
 }
 
-// ---- tensor contracts -------------------------------------------------------------------------
-bool present(const ep_tensor_t& t) { return t.data != nullptr; }
-
-int elem_size(int dtype) {
-    switch (dtype) {
-        case EP_DTYPE_BF16: case EP_DTYPE_I16: return 2;
-        case EP_DTYPE_FP8_E4M3: case EP_DTYPE_U8: return 1;
-        case EP_DTYPE_I32: case EP_DTYPE_F32: return 4;
-        case EP_DTYPE_I64: return 8;
-        default: return 0;
-    }
-}
-
-bool contiguous(const ep_tensor_t& t) {
-    int64_t expect = 1;
-    for (int d = t.ndim - 1; d >= 0; --d) {
-        if (t.size[d] != 1 && t.stride[d] != expect) return false;
-        expect *= t.size[d];
-    }
-    return true;
-}
-
 }  // namespace
+
+static std::string library_dir() {
+    Dl_info info;
+    if (dladdr((void*)&library_dir, &info) == 0 || info.dli_fname == nullptr) return ".";
+    std::string p = info.dli_fname;
+    const auto pos = p.find_last_of('/');
+    return pos == std::string::npos ? "." : p.substr(0, pos);
+}
+
+std::string ep_code_object_path(const char* dir, const char* name) {
+    const std::string path = (dir != nullptr ? std::string(dir) : library_dir()) + "/" + name;
+    FILE* f = fopen(path.c_str(), "rb");
+    if (f == nullptr) throw EpError{"cannot open the gfx950 code object " + path + " (build it first)"};
+    fclose(f);
+    return path;
+}
+
+void ep_set_last_error(const char* message) { g_err = message; }
 
 struct ep_buffer {
     int rank_idx = 0, num_ranks = 1;
@@ -616,6 +555,7 @@ const char* ep_last_error(void) { return g_err.c_str(); }
 int ep_init(const char* dir) {
     return guarded([&] {
         load_kernels(dir);
+        ep_load_expert_kernels(dir);
         ep_static_scratch_init();      // the address of the static scratch on this device
     });
 }

@@ -561,6 +561,127 @@ private:
     bool exact_sync_sizes_ = false;
 };
 
+// ---- the experts' computation (deep_ep/experts.py checks what the C ABI does not see: devices, overlapping kinds of arguments) ----
+
+// Matrices of the experts, [E, N, K], or one matrix: what the C ABI takes of expert 0, and the stride between experts.
+ep_tensor_t expert_matrix(const at::Tensor& t, int64_t& expert_stride) {
+    EP_PY_ASSERT(t.dim() == 2 || t.dim() == 3);
+    if (t.dim() == 2) {
+        expert_stride = 0;
+        return desc(t);
+    }
+    ep_tensor_t d{};
+    d.data = t.data_ptr() != nullptr ? t.data_ptr() : nonnull_ptr(t);
+    d.dtype = dtype_code(t, false);
+    d.ndim = 2;
+    for (int i = 0; i < 2; ++i) {
+        d.size[i] = t.size(i + 1);
+        d.stride[i] = t.stride(i + 1);
+    }
+    expert_stride = t.size(0) > 1 ? t.stride(0) : 0;
+    return d;
+}
+int num_matrices(const at::Tensor& t) { return t.dim() == 3 ? (int)t.size(0) : 1; }
+
+// Kernels run on the current device: everything they are given has to be there.
+void on_current_device(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && !t->is_cuda()) throw EpPyError("every tensor handed to the EP kernels must live on the GPU");
+    const int current = c10::hip::getCurrentHIPStream().device_index();
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->device().index() != current)
+            throw EpPyError("every tensor handed to the EP kernels must live on the current device");
+}
+const at::Tensor* of(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
+
+at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf, const OptTensor& psum,
+                          int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
+    on_current_device({&x, of(x_sf), &weight, of(weight_sf), of(psum), of(out)});
+    EP_PY_ASSERT(x.dim() == 2);
+    ep_grouped_linear_args_t a{};
+    a.x = desc(x);
+    a.x_sf = desc(x_sf);
+    a.weight = expert_matrix(weight, a.weight_expert_stride);
+    if (weight_sf.has_value()) {
+        EP_PY_ASSERT(weight_sf->dim() == weight.dim() && num_matrices(*weight_sf) == num_matrices(weight));
+        a.weight_sf = expert_matrix(*weight_sf, a.weight_sf_expert_stride);
+    }
+    a.psum_num_recv_tokens_per_expert = desc(psum);
+    const at::Tensor y = out.has_value() ? *out : alloc({x.size(0), weight.size(transpose_weight ? -1 : -2)}, at::kBFloat16, x.device());
+    a.out = desc(y);
+    a.num_experts = num_matrices(weight);
+    a.expert_alignment = alignment;
+    a.zero_rows = zero_rows;
+    a.transpose_weight = transpose_weight;
+    a.stream = current_stream();
+    check(ep_grouped_linear(&a));
+    return y;
+}
+
+at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, const OptTensor& psum, int num_experts, int alignment,
+                               const OptTensor& out, bool accumulate) {
+    on_current_device({&grad, &x, of(psum), of(out)});
+    EP_PY_ASSERT(grad.dim() == 2 && x.dim() == 2);
+    const at::Tensor w = out.has_value() ? *out : alloc({num_experts, grad.size(1), x.size(1)}, at::kBFloat16, x.device());
+    ep_grouped_weight_grad_args_t a{};
+    a.grad = desc(grad);
+    a.x = desc(x);
+    a.psum_num_recv_tokens_per_expert = desc(psum);
+    a.out = expert_matrix(w, a.out_expert_stride);
+    EP_PY_ASSERT(num_matrices(w) == num_experts);
+    a.num_experts = num_experts;
+    a.expert_alignment = alignment;
+    a.accumulate = accumulate;
+    a.stream = current_stream();
+    check(ep_grouped_weight_grad(&a));
+    return w;
+}
+
+std::tuple<at::Tensor, OptTensor> swiglu(const at::Tensor& h, const OptTensor& weights, const OptTensor& psum, int num_experts, int alignment,
+                                         bool quantise, const OptTensor& out, const OptTensor& out_sf, int zero_rows) {
+    on_current_device({&h, of(weights), of(psum), of(out), of(out_sf)});
+    EP_PY_ASSERT(h.dim() == 2);
+    const int64_t rows = h.size(0), channels = h.size(1) / 2;
+    const at::Tensor y = out.has_value() ? *out : alloc({rows, channels}, quantise ? at::kFloat8_e4m3fn : at::kBFloat16, h.device());
+    OptTensor sf = out_sf;
+    if (quantise && !sf.has_value()) sf = alloc({rows, (channels + 127) / 128}, at::kFloat, h.device());
+    EP_PY_ASSERT(y.scalar_type() == (quantise ? at::kFloat8_e4m3fn : at::kBFloat16));
+    ep_swiglu_args_t a{};
+    a.h = desc(h);
+    a.weights = desc(weights);
+    a.psum_num_recv_tokens_per_expert = desc(psum);
+    a.out = desc(y);
+    a.out_sf = desc(sf);
+    a.num_experts = num_experts;
+    a.expert_alignment = alignment;
+    a.zero_rows = zero_rows;
+    a.stream = current_stream();
+    check(ep_swiglu(&a));
+    return {y, sf};
+}
+
+std::tuple<at::Tensor, OptTensor> swiglu_grad(const at::Tensor& grad, const at::Tensor& h, const OptTensor& weights, const OptTensor& psum,
+                                              int num_experts, int alignment, int zero_rows) {
+    on_current_device({&grad, &h, of(weights), of(psum)});
+    EP_PY_ASSERT(h.dim() == 2 && grad.dim() == 2);
+    const at::Tensor grad_h = alloc({h.size(0), h.size(1)}, at::kBFloat16, h.device());
+    OptTensor grad_weights;
+    if (weights.has_value()) grad_weights = alloc({h.size(0)}, at::kFloat, h.device());
+    ep_swiglu_grad_args_t a{};
+    a.grad = desc(grad);
+    a.h = desc(h);
+    a.weights = desc(weights);
+    a.psum_num_recv_tokens_per_expert = desc(psum);
+    a.grad_h = desc(grad_h);
+    a.grad_weights = desc(grad_weights);
+    a.num_experts = num_experts;
+    a.expert_alignment = alignment;
+    a.zero_rows = zero_rows;
+    a.stream = current_stream();
+    check(ep_swiglu_grad(&a));
+    return {grad_h, grad_weights};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -570,6 +691,10 @@ PYBIND11_MODULE(_native, m) {
         const auto stream = c10::hip::getCurrentHIPStream();
         return py::make_tuple((int64_t)stream.id(), (int)stream.device_index(), (int)stream.unwrap().device_type());
     }, "(stream_id, device_index, device_type) of the current stream");
+    m.def("grouped_linear", &grouped_linear);
+    m.def("grouped_weight_grad", &grouped_weight_grad);
+    m.def("swiglu", &swiglu);
+    m.def("swiglu_grad", &swiglu_grad);
     py::class_<LaunchEvent>(m, "LaunchEvent")
         .def("current_stream_wait", &LaunchEvent::current_stream_wait)
         .def_property_readonly("handle", &LaunchEvent::handle)

@@ -1,6 +1,7 @@
 """Builds the native artefacts of the package for gfx950, in-tree:
 
   deep_ep/lib/ep_kernels.hsaco     device code object   (hipcc --genco)
+  deep_ep/lib/ep_experts.hsaco     device code object of the experts' computation
   deep_ep/lib/libdeep_ep_hip.so    host runtime, C ABI  (hipcc -shared)
   deep_ep/_native.*.so             compiled Python binding of dispatch/combine over that C ABI  (g++, pybind11 + torch headers)
   deep_ep/lib/abi_client           a plain-C caller of the C ABI, used by the tests  (gcc)
@@ -55,7 +56,9 @@ def run(cmd):
 def build(verbose: bool = True) -> None:
     os.makedirs(LIB, exist_ok=True)
     run([HIPCC, *DEVICE_FLAGS, '-o', os.path.join(LIB, 'ep_kernels.hsaco'), os.path.join(CSRC, 'ep_kernels.hip')])
-    run([HIPCC, *HOST_FLAGS, '-o', os.path.join(LIB, 'libdeep_ep_hip.so'), os.path.join(CSRC, 'ep_runtime.cpp')])
+    run([HIPCC, *DEVICE_FLAGS, '-o', os.path.join(LIB, 'ep_experts.hsaco'), os.path.join(CSRC, 'ep_experts.hip')])
+    run([HIPCC, *HOST_FLAGS, '-o', os.path.join(LIB, 'libdeep_ep_hip.so'), os.path.join(CSRC, 'ep_runtime.cpp'),
+         os.path.join(CSRC, 'ep_experts.cpp')])
     run(binding_command())
     os.makedirs(CALIB_LIB, exist_ok=True)
     run([HIPCC, *DEVICE_FLAGS, '-o', os.path.join(CALIB_LIB, 'ep_calib.hsaco'), os.path.join(CSRC, 'ep_calib.hip')])

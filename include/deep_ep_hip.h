@@ -310,6 +310,75 @@ int ep_combine_launch(ep_buffer_t* buf, const ep_combine_args_t* args, int phase
 /* Phase 0 with an event behind it (see ep_dispatch_launch_event). */
 int ep_combine_begin_event(ep_buffer_t* buf, const ep_combine_args_t* args, void* event);
 
+/* ---- the experts' computation ----------------------------------------------------------------- */
+
+/* What lies between a dispatch and a combine: products of every expert's rows with that expert's weights, their
+ * gradients, the gated activation.  No counterpart in the reference, which leaves the experts to its callers.
+ *
+ * The rows' layout is the dispatch's: psum_num_recv_tokens_per_expert [E] int32 on the device and the expert alignment
+ * say which rows are an expert's (from align(psum[e - 1]) up to psum[e]); without a psum (absent) one expert has all rows.
+ * Counts are read on the device only: nothing waits for the host, and rows that the counts place outside the tensors are
+ * left out.  Rows of no expert (padding, and what lies behind the last expert's) take no part: they are read for
+ * nothing and stay as they were in the results, or become zeros as zero_rows says.  Sums are held in 32 bits and rounded once.  Rows are addressed with their stride; channels are
+ * contiguous, start on 16 bytes and come in multiples of 8 (BF16) or 16 (FP8 depth). */
+/* zero_rows: which rows of no expert are written, as zeros */
+enum ep_zero_rows {
+    EP_ZERO_NONE = 0,
+    EP_ZERO_PADDING = 1,                /* behind every expert's rows up to the next multiple of the alignment */
+    EP_ZERO_ALL = 2                     /* and everything behind the last expert's */
+};
+
+typedef struct ep_grouped_linear_args {
+    ep_tensor_t x;                      /* [M,K] BF16, or e4m3fn with x_sf */
+    ep_tensor_t x_sf;                   /* [M, ceil(K/128)] fp32, any strides */
+    ep_tensor_t weight;                 /* [N,K] of expert 0 ([K,N] if transpose_weight), dtype of x */
+    ep_tensor_t weight_sf;              /* [ceil(N/128), ceil(K/128)] fp32 of expert 0 (FP8) */
+    ep_tensor_t psum_num_recv_tokens_per_expert;        /* [E] int32 (absent: one expert has all rows) */
+    ep_tensor_t out;                    /* [M,N] BF16 */
+    int64_t weight_expert_stride, weight_sf_expert_stride;      /* elements */
+    int32_t num_experts, expert_alignment, zero_rows;
+    int32_t transpose_weight;           /* the product with the transposed weights (gradient of the rows), BF16 */
+    void* stream;
+} ep_grouped_linear_args_t;
+/* out[m] = W[e(m)] x[m].  FP8: sums over groups of 128 channels, each scaled by x_sf[m,g] * weight_sf[e(m),n/128,g]. */
+int ep_grouped_linear(const ep_grouped_linear_args_t* args);
+
+typedef struct ep_grouped_weight_grad_args {
+    ep_tensor_t grad;                   /* [M,N] BF16: gradient of the result */
+    ep_tensor_t x;                      /* [M,K] BF16 */
+    ep_tensor_t psum_num_recv_tokens_per_expert;
+    ep_tensor_t out;                    /* [N,K] of expert 0, BF16 or fp32 */
+    int64_t out_expert_stride;          /* elements */
+    int32_t num_experts, expert_alignment;
+    int32_t accumulate;                 /* fp32: added to what is there */
+    void* stream;
+} ep_grouped_weight_grad_args_t;
+/* out[e] = sum over the rows m of expert e of grad[m] x[m]^T; zeros for an expert without rows. */
+int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args);
+
+typedef struct ep_swiglu_args {
+    ep_tensor_t h;                      /* [M,2I] BF16: gates, then ups */
+    ep_tensor_t weights;                /* [M] fp32 (optional): gate weight of the row */
+    ep_tensor_t psum_num_recv_tokens_per_expert;
+    ep_tensor_t out;                    /* [M,I] BF16, or e4m3fn with out_sf */
+    ep_tensor_t out_sf;                 /* [M, ceil(I/128)] fp32, any strides */
+    int32_t num_experts, expert_alignment, zero_rows;
+    void* stream;
+} ep_swiglu_args_t;
+/* out[m] = silu(gate[m]) * up[m] * weights[m]; quantised as ep_per_token_cast_to_fp8 does, without a rounding to BF16 between. */
+int ep_swiglu(const ep_swiglu_args_t* args);
+
+typedef struct ep_swiglu_grad_args {
+    ep_tensor_t grad;                   /* [M,I] BF16: gradient of the result */
+    ep_tensor_t h, weights;             /* as above */
+    ep_tensor_t psum_num_recv_tokens_per_expert;
+    ep_tensor_t grad_h;                 /* [M,2I] BF16 out */
+    ep_tensor_t grad_weights;           /* [M] fp32 out (optional) */
+    int32_t num_experts, expert_alignment, zero_rows;
+    void* stream;
+} ep_swiglu_grad_args_t;
+int ep_swiglu_grad(const ep_swiglu_grad_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif

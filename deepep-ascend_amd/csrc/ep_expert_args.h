@@ -4,11 +4,24 @@
 
 #define EP_EXPERT_MAX_DEPTH_FP8 32768      // channels of an FP8 row: the scales of a column block fit a table in LDS
 
+#define EP_LORA_STEP 512                   // channels that a workgroup of ep_lora_down_* goes through at a time
+
 // Rows of the expert-major layout: expert e has rows [align(psum[e - 1]), psum[e]); psum == nullptr: one expert has all rows.
 struct EpExpertLayout {
     const int* psum;
     int num_experts, alignment, num_rows;
     int zero_rows;                // EP_ZERO_*: which rows of no expert are written, as zeros
+};
+
+// Low-rank adapters beside a product: out[r] += up[a][e] low[r], low[r] = scale[a] down[a][e] rows[r] with a = adapter[r].
+struct EpLoraArgs {
+    const int* adapter;           // [rows]; outside [0, num_adapters): none
+    const char *down, *up;        // BF16: [rank, depth] and [columns, rank] of adapter 0 and expert 0
+    int64_t down_ld, down_adapter, down_expert, up_ld, up_adapter, up_expert;     // bytes
+    const float* scales;          // [num_adapters] or nullptr
+    float* low;                   // [chunks, rows, rank]: sums over the chunks of the depth
+    int num_adapters, rank, chunks;
+    int chunk_depth, slots;       // the launch in front: channels of a chunk, workgroups that share a tile's adapters
 };
 
 // out[r, c] = sum_d rows[r, d] columns[c, d] over a tile of output rows and output columns.
@@ -26,6 +39,15 @@ struct EpGemmArgs {
     int num_out_rows;             // weight gradient: rows of the output of one expert
     int column_tiles, row_tiles;  // (row_tiles: weight gradient)
     int accumulate;               // weight gradient in 32 bits: added to what is there
+    EpLoraArgs lora;
+};
+
+struct EpExpandIndexArgs {
+    const int* metadata;          // [rows, topk + 2]
+    const int* psum_rank;         // [ranks]
+    const int* values;
+    int* out;
+    int num_rows, num_ranks, topk, num_values, num_out;
 };
 
 struct EpSwigluArgs {

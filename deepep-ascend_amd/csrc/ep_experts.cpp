@@ -12,7 +12,8 @@ namespace {
 struct ExpertKernels {
     hipModule_t module = nullptr;
     int device = -1;
-    hipFunction_t bf16, fp8, transposed, weights[2], swiglu[2], swiglu_grad;
+    hipFunction_t bf16, fp8, transposed, lora, weights[2], swiglu[2], swiglu_grad;
+    hipFunction_t lora_down[2][3], expand_fill, expand_rows;
 };
 ExpertKernels g_k;
 std::mutex g_mutex;
@@ -89,6 +90,11 @@ void ep_load_expert_kernels(const char* dir) {
     get(g_k.bf16, "ep_grouped_bf16");
     get(g_k.fp8, "ep_grouped_fp8");
     get(g_k.transposed, "ep_grouped_transposed_bf16");
+    get(g_k.lora, "ep_grouped_lora_bf16");
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 3; ++j) get(g_k.lora_down[i][j], format("ep_lora_down_%d_%d", 16 << i, 16 << j).c_str());
+    get(g_k.expand_fill, "ep_expand_fill");
+    get(g_k.expand_rows, "ep_expand_token_index_rows");
     get(g_k.weights[0], "ep_grouped_weights_bf16");
     get(g_k.weights[1], "ep_grouped_weights_f32");
     get(g_k.swiglu[0], "ep_swiglu_bf16");
@@ -99,54 +105,155 @@ void ep_load_expert_kernels(const char* dir) {
 
 extern "C" {
 
+// The arguments of a product of rows, checked.
+static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
+    const ep_tensor_t &x = args->x, &w = args->weight, &out = args->out;
+    EP_HOST_ASSERT(row_major(x) and addressable(x));
+    EP_HOST_ASSERT(row_major(w) and addressable(w) and w.dtype == x.dtype);
+    const bool fp8 = x.dtype == EP_DTYPE_FP8_E4M3, transposed = args->transpose_weight != 0;
+    EP_HOST_ASSERT(fp8 or x.dtype == EP_DTYPE_BF16);
+    EP_HOST_ASSERT(not (fp8 and transposed));
+    const int64_t rows = x.size[0], depth = x.size[1], columns = w.size[transposed ? 1 : 0];
+    EP_HOST_ASSERT(w.size[transposed ? 0 : 1] == depth);
+    EP_HOST_ASSERT(depth % (fp8 ? 16 : 8) == 0 and columns > 0 and columns % 8 == 0);
+    EP_HOST_ASSERT(depth <= INT32_MAX / 2 and columns <= INT32_MAX / 2);
+    EP_HOST_ASSERT(args->num_experts == 1 or (args->weight_expert_stride >= 0 and args->weight_expert_stride * elem_size(w.dtype) % 16 == 0));
+    EP_HOST_ASSERT(row_major(out) and out.dtype == EP_DTYPE_BF16);
+    EP_HOST_ASSERT(out.size[0] == rows and out.size[1] == columns);
+    EpGemmArgs g{};
+    g.layout = layout_of(args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment, args->zero_rows, rows);
+    g.rows = (const char*)x.data;
+    g.columns = (const char*)w.data;
+    g.rows_ld = row_stride(x) * elem_size(x.dtype);
+    g.columns_ld = row_stride(w) * elem_size(w.dtype);
+    g.columns_expert = args->weight_expert_stride * elem_size(w.dtype);
+    g.out = (char*)out.data;
+    g.out_ld = row_stride(out);
+    g.depth = (int)depth;
+    g.num_columns = (int)columns;
+    EP_HOST_ASSERT(fp8 == present(args->x_sf) and fp8 == present(args->weight_sf));
+    if (fp8) {
+        const ep_tensor_t &sf = args->x_sf, &wsf = args->weight_sf;
+        EP_HOST_ASSERT(depth <= EP_EXPERT_MAX_DEPTH_FP8);
+        EP_HOST_ASSERT(sf.ndim == 2 and sf.dtype == EP_DTYPE_F32 and sf.size[0] == rows and sf.size[1] == ceil_div(depth, 128));
+        EP_HOST_ASSERT(sf.stride[0] >= 0 and sf.stride[1] >= 0 and (rows <= 1 or sf.stride[0] * 4 <= kMaxRowBytes));
+        EP_HOST_ASSERT(wsf.ndim == 2 and wsf.dtype == EP_DTYPE_F32);
+        EP_HOST_ASSERT(wsf.size[0] == ceil_div(columns, 128) and wsf.size[1] == ceil_div(depth, 128));
+        g.rows_sf = (const float*)sf.data;
+        g.columns_sf = (const float*)wsf.data;
+        g.rows_sf_row = rows > 1 ? sf.stride[0] : 1;
+        g.rows_sf_col = sf.stride[1];
+        g.columns_sf_row = wsf.stride[0];
+        g.columns_sf_col = wsf.stride[1];
+        g.columns_sf_expert = args->weight_sf_expert_stride;
+    }
+    g.column_tiles = (int)ceil_div(columns, kTile);
+    return g;
+}
+
 int ep_grouped_linear(const ep_grouped_linear_args_t* args) {
     return guarded([&] {
         EP_HOST_ASSERT(args != nullptr);
-        const ep_tensor_t &x = args->x, &w = args->weight, &out = args->out;
-        EP_HOST_ASSERT(row_major(x) and addressable(x));
-        EP_HOST_ASSERT(row_major(w) and addressable(w) and w.dtype == x.dtype);
-        const bool fp8 = x.dtype == EP_DTYPE_FP8_E4M3, transposed = args->transpose_weight != 0;
-        EP_HOST_ASSERT(fp8 or x.dtype == EP_DTYPE_BF16);
-        EP_HOST_ASSERT(not (fp8 and transposed));
-        const int64_t rows = x.size[0], depth = x.size[1], columns = w.size[transposed ? 1 : 0];
-        EP_HOST_ASSERT(w.size[transposed ? 0 : 1] == depth);
-        EP_HOST_ASSERT(depth % (fp8 ? 16 : 8) == 0 and columns > 0 and columns % 8 == 0);
-        EP_HOST_ASSERT(depth <= INT32_MAX / 2 and columns <= INT32_MAX / 2);
-        EP_HOST_ASSERT(args->num_experts == 1 or (args->weight_expert_stride >= 0 and args->weight_expert_stride * elem_size(w.dtype) % 16 == 0));
-        EP_HOST_ASSERT(row_major(out) and out.dtype == EP_DTYPE_BF16);
-        EP_HOST_ASSERT(out.size[0] == rows and out.size[1] == columns);
-        EpGemmArgs g{};
-        g.layout = layout_of(args->psum_num_recv_tokens_per_expert, args->num_experts, args->expert_alignment, args->zero_rows, rows);
-        g.rows = (const char*)x.data;
-        g.columns = (const char*)w.data;
-        g.rows_ld = row_stride(x) * elem_size(x.dtype);
-        g.columns_ld = row_stride(w) * elem_size(w.dtype);
-        g.columns_expert = args->weight_expert_stride * elem_size(w.dtype);
-        g.out = (char*)out.data;
-        g.out_ld = row_stride(out);
-        g.depth = (int)depth;
-        g.num_columns = (int)columns;
-        EP_HOST_ASSERT(fp8 == present(args->x_sf) and fp8 == present(args->weight_sf));
-        if (fp8) {
-            const ep_tensor_t &sf = args->x_sf, &wsf = args->weight_sf;
-            EP_HOST_ASSERT(depth <= EP_EXPERT_MAX_DEPTH_FP8);
-            EP_HOST_ASSERT(sf.ndim == 2 and sf.dtype == EP_DTYPE_F32 and sf.size[0] == rows and sf.size[1] == ceil_div(depth, 128));
-            EP_HOST_ASSERT(sf.stride[0] >= 0 and sf.stride[1] >= 0 and (rows <= 1 or sf.stride[0] * 4 <= kMaxRowBytes));
-            EP_HOST_ASSERT(wsf.ndim == 2 and wsf.dtype == EP_DTYPE_F32);
-            EP_HOST_ASSERT(wsf.size[0] == ceil_div(columns, 128) and wsf.size[1] == ceil_div(depth, 128));
-            g.rows_sf = (const float*)sf.data;
-            g.columns_sf = (const float*)wsf.data;
-            g.rows_sf_row = rows > 1 ? sf.stride[0] : 1;
-            g.rows_sf_col = sf.stride[1];
-            g.columns_sf_row = wsf.stride[0];
-            g.columns_sf_col = wsf.stride[1];
-            g.columns_sf_expert = args->weight_sf_expert_stride;
-        }
-        if (rows == 0) return;
-        g.column_tiles = (int)ceil_div(columns, kTile);
+        EpGemmArgs g = linear_args(args);
+        if (g.layout.num_rows == 0) return;
         const ExpertKernels& k = kernels();
-        launch(fp8 ? k.fp8 : transposed ? k.transposed : k.bf16, align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256,
-               args->stream, g);
+        launch(args->x.dtype == EP_DTYPE_FP8_E4M3 ? k.fp8 : args->transpose_weight ? k.transposed : k.bf16,
+               align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256, args->stream, g);
+    });
+}
+
+// How the rows times the adapters' first matrices are split: rows of a workgroup's tile, chunks of the depth, workgroups that share the
+// adapters of a tile.
+struct LoraPlan {
+    int rows, chunks, chunk_depth, slots;
+};
+static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
+    LoraPlan p{};
+    p.rows = rows <= 2048 ? 16 : 32;
+    const int64_t tiles = std::max<int64_t>(1, rows / p.rows + std::min<int64_t>(num_experts, rows));
+    p.slots = (int)std::clamp<int64_t>(ceil_div(512, tiles), 1, std::min<int64_t>(p.rows, std::max<int64_t>(rows, 1)));
+    const int64_t steps = ceil_div(depth, EP_LORA_STEP), chunks = std::clamp<int64_t>(ceil_div(512, tiles * p.slots), 1, std::min<int64_t>(steps, 16));
+    p.chunk_depth = (int)(ceil_div(steps, chunks) * EP_LORA_STEP);
+    p.chunks = (int)ceil_div(depth, p.chunk_depth);
+    return p;
+}
+
+int64_t ep_grouped_lora_workspace_bytes(int64_t num_rows, int num_experts, int64_t depth, int rank) {
+    if (num_rows < 0 or num_rows > INT32_MAX or num_experts <= 0 or depth <= 0 or depth > INT32_MAX / 2 or rank <= 0 or rank > EP_LORA_MAX_RANK) return -1;
+    return lora_plan(num_rows, num_experts, depth).chunks * num_rows * rank * 4;
+}
+
+int ep_grouped_lora_linear(const ep_grouped_lora_args_t* args) {
+    return guarded([&] {
+        EP_HOST_ASSERT(args != nullptr);
+        EpGemmArgs g = linear_args(&args->linear);
+        EP_HOST_ASSERT(args->linear.x.dtype == EP_DTYPE_BF16 and args->linear.transpose_weight == 0);
+        const ep_tensor_t &down = args->lora_a, &up = args->lora_b, &idx = args->adapter_idx, &scales = args->scales;
+        EP_HOST_ASSERT(row_major(down) and down.dtype == EP_DTYPE_BF16 and addressable(down));
+        EP_HOST_ASSERT(row_major(up) and up.dtype == EP_DTYPE_BF16 and addressable(up));
+        const int64_t rank = down.size[0];
+        EP_HOST_ASSERT(rank > 0 and rank % 8 == 0 and rank <= EP_LORA_MAX_RANK);
+        EP_HOST_ASSERT(down.size[1] == g.depth and up.size[0] == g.num_columns and up.size[1] == rank);
+        EP_HOST_ASSERT(args->num_adapters > 0);
+        for (const int64_t stride : {args->lora_a_adapter_stride, args->lora_a_expert_stride, args->lora_b_adapter_stride, args->lora_b_expert_stride})
+            EP_HOST_ASSERT(stride >= 0 and stride % 8 == 0);
+        EP_HOST_ASSERT(present(idx) and idx.ndim == 1 and idx.dtype == EP_DTYPE_I32 and contiguous(idx) and idx.size[0] == g.layout.num_rows);
+        if (present(scales)) {
+            EP_HOST_ASSERT(scales.ndim == 1 and scales.dtype == EP_DTYPE_F32 and contiguous(scales) and scales.size[0] == args->num_adapters);
+        }
+        const LoraPlan plan = lora_plan(g.layout.num_rows, g.layout.num_experts, g.depth);
+        const int64_t bytes = (int64_t)plan.chunks * g.layout.num_rows * rank * 4;
+        EP_HOST_ASSERT(bytes == 0 or (args->workspace != nullptr and ((uintptr_t)args->workspace & 15) == 0));
+        EP_HOST_ASSERT(args->workspace_bytes >= bytes);
+        if (g.layout.num_rows == 0) return;
+        EpLoraArgs& l = g.lora;
+        l.adapter = (const int*)idx.data;
+        l.down = (const char*)down.data;
+        l.up = (const char*)up.data;
+        l.down_ld = row_stride(down) * 2;
+        l.down_adapter = args->lora_a_adapter_stride * 2;
+        l.down_expert = args->lora_a_expert_stride * 2;
+        l.up_ld = row_stride(up) * 2;
+        l.up_adapter = args->lora_b_adapter_stride * 2;
+        l.up_expert = args->lora_b_expert_stride * 2;
+        l.scales = (const float*)scales.data;
+        l.low = (float*)args->workspace;
+        l.num_adapters = args->num_adapters;
+        l.rank = (int)rank;
+        l.chunks = plan.chunks;
+        l.chunk_depth = plan.chunk_depth;
+        l.slots = plan.slots;
+        const ExpertKernels& k = kernels();
+        const int64_t tiles = row_tiles_bound(g.layout, plan.rows);
+        launch(k.lora_down[plan.rows == 16 ? 0 : 1][rank <= 16 ? 0 : rank <= 32 ? 1 : 2], tiles * plan.chunks * plan.slots, 256,
+               args->linear.stream, g);
+        launch(k.lora, align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256, args->linear.stream, g);
+    });
+}
+
+int ep_expand_token_index(const ep_tensor_t* values, const ep_tensor_t* src_metadata, const ep_tensor_t* psum_num_recv_tokens_per_rank,
+                          const ep_tensor_t* out, void* stream) {
+    return guarded([&] {
+        EP_HOST_ASSERT(values != nullptr and src_metadata != nullptr and psum_num_recv_tokens_per_rank != nullptr and out != nullptr);
+        const ep_tensor_t &v = *values, &m = *src_metadata, &psum = *psum_num_recv_tokens_per_rank, &o = *out;
+        for (const ep_tensor_t* t : {&v, &m, &psum, &o})
+            EP_HOST_ASSERT(present(*t) and t->dtype == EP_DTYPE_I32 and contiguous(*t) and t->size[0] <= INT32_MAX);
+        EP_HOST_ASSERT(v.ndim == 1 and m.ndim == 2 and psum.ndim == 1 and o.ndim == 1);
+        EP_HOST_ASSERT(m.size[1] > 2 and m.size[1] <= INT32_MAX and psum.size[0] > 0);
+        EpExpandIndexArgs e{};
+        e.metadata = (const int*)m.data;
+        e.psum_rank = (const int*)psum.data;
+        e.values = (const int*)v.data;
+        e.out = (int*)o.data;
+        e.num_rows = (int)m.size[0];
+        e.num_ranks = (int)psum.size[0];
+        e.topk = (int)m.size[1] - 2;
+        e.num_values = (int)v.size[0];
+        e.num_out = (int)o.size[0];
+        if (e.num_out == 0) return;
+        const ExpertKernels& k = kernels();
+        launch(k.expand_fill, ceil_div(e.num_out, 256), 256, stream, e);
+        if (e.num_rows > 0) launch(k.expand_rows, ceil_div((int64_t)e.num_rows * e.topk, 256), 256, stream, e);
     });
 }
 

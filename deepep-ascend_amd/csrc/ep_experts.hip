@@ -237,11 +237,39 @@ union Fragment8 {
     i32x8 v;
 };
 
+// ---- low-rank adapters: numbers of a tile ------------------------------------------------------------------
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) v = min(v, __shfl_xor(v, d));
+    return v;
+}
+constexpr int NO_ADAPTER = 0x7fffffff;
+// The smallest number of the tile's rows above `last`; every wave finds it by itself.
+template <int TM>
+__device__ __forceinline__ int next_adapter(const int* of_row, int last) {
+    int v = NO_ADAPTER;
+#pragma unroll
+    for (int i = 0; i < TM; i += WAVE) {
+        const int r = i + lane_id();
+        const int a = r < TM ? of_row[r] : NO_ADAPTER;
+        v = min(v, a > last ? a : NO_ADAPTER);
+    }
+    return uniform(wave_min(v));
+}
+template <int TM>
+__device__ __forceinline__ void note_adapters(const EpLoraArgs& l, int first, int valid, int* of_row, int threads) {
+    for (int r = threadIdx.x; r < TM; r += threads) {
+        const int a = r < valid ? l.adapter[first + r] : -1;
+        of_row[r] = a >= 0 && a < l.num_adapters ? a : NO_ADAPTER;
+    }
+}
+
 // ---- products ---------------------------------------------------------------------------------------------
 //
 // One workgroup computes TM x TN of the output, WR x WC waves a part each, in 32 bits.  The matrix instruction's first operand is
 // the output's columns, its second the rows: a lane then holds four neighbouring columns of one row.
-template <int TM, int TN, int WR, int WC, int STAGES, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32>
+template <int TM, int TN, int WR, int WC, int STAGES, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false>
 struct Gemm {
     static constexpr int WAVES = WR * WC, FM = TM / WR, FN = TN / WC, NR = FM / 16, NC = FN / 16;
     static constexpr int COLUMNS_BYTES = TN * 128, ROWS_BYTES = TM * 128, SF_BYTES = FP8 ? (TM < WAVE ? WAVE : TM) * 4 : 0;
@@ -257,9 +285,11 @@ struct Gemm {
 
     // rows .. rows + valid: what is computed, up to limit zeros are written; columns from column on
     __device__ __forceinline__ static void run(const EpGemmArgs& a, const char* rows, const char* columns, int valid, int limit,
-                                               int num_columns, int depth, const float* rows_sf, const float* columns_sf, char* out) {
+                                               int num_columns, int depth, const float* rows_sf, const float* columns_sf, char* out,
+                                               int first = 0, const char* up = nullptr) {
         __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];
         __shared__ float table[FP8 ? BLOCKS * TABLE : 1];
+        __shared__ int adapters[LORA ? TM : 1];
         const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
         const int first_row = (wave / WC) * FM, first_column = (wave % WC) * FN;
         const unsigned lds0 = (unsigned)(size_t)(lds_byte*)lds;
@@ -297,10 +327,28 @@ struct Gemm {
             }
         };
 
+        auto multiply = [&](const char* at, const char* at_rows) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                u32x4 c[NC], r[NR];
+#pragma unroll
+                for (int j = 0; j < NC; ++j) c[j] = fragment<COLUMNS_T, TN>(at, first_column + j * 16, half);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) r[i] = fragment<ROWS_T, TM>(at_rows, first_row + i * 16, half);
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c[j]), __builtin_bit_cast(bf16x8, r[i]),
+                                                                           acc[i][j], 0, 0, 0);
+            }
+        };
+
         if (steps > 0) {
 #pragma unroll
             for (int s = 0; s < STAGES - 1; ++s) fetch(s, s);
         }
+        if (LORA) add_adapters(a, lds + (STAGES - 1) * STAGE_BYTES, adapters, first, valid, num_columns, up, multiply);
         int stage = 0;
         for (int s = 0; s < steps; ++s) {
             wait_and_meet<(STAGES - 2) * FETCHES>();
@@ -308,20 +356,7 @@ struct Gemm {
             const char* const at = lds + stage * STAGE_BYTES;
             const char* const at_rows = at + COLUMNS_BYTES;
             if (!FP8) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    u32x4 c[NC], r[NR];
-#pragma unroll
-                    for (int j = 0; j < NC; ++j) c[j] = fragment<COLUMNS_T, TN>(at, first_column + j * 16, half);
-#pragma unroll
-                    for (int i = 0; i < NR; ++i) r[i] = fragment<ROWS_T, TM>(at_rows, first_row + i * 16, half);
-#pragma unroll
-                    for (int i = 0; i < NR; ++i)
-#pragma unroll
-                        for (int j = 0; j < NC; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c[j]), __builtin_bit_cast(bf16x8, r[i]),
-                                                                               acc[i][j], 0, 0, 0);
-                }
+                multiply(at, at_rows);
             } else {
                 // a step is one group of channels: its products are summed by themselves, then scaled
                 const float* const scales = (const float*)(at_rows + ROWS_BYTES);
@@ -379,6 +414,56 @@ struct Gemm {
         }
     }
 
+    // The adapters' part, in front of the product's first step and in the LDS of its last stage, while the first ones are on their way: for
+    // every adapter that rows of the tile have, 32 ranks at a time, a step of 64 channels.  The low-rank rows are sums in 32 bits; they
+    // go in as two BF16, the rounded value and the rest, against the same column of `up` twice, which keeps 2^-17 of them.
+    template <typename Multiply>
+    __device__ __forceinline__ static void add_adapters(const EpGemmArgs& a, char* stage, int* of_row, int first, int valid, int num_columns,
+                                                        const char* up, Multiply multiply) {
+        constexpr int THREADS = WAVES * WAVE;
+        const EpLoraArgs& l = a.lora;
+        char* const to_columns = stage;
+        char* const to_rows = stage + COLUMNS_BYTES;
+        note_adapters<TM>(l, first, valid, of_row, THREADS);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int number = next_adapter<TM>(of_row, -1); number != NO_ADAPTER; number = next_adapter<TM>(of_row, number)) {
+            for (int r0 = 0; r0 < l.rank; r0 += 32) {
+                for (int i = threadIdx.x; i < TM * 4; i += THREADS) {
+                    const int r = i >> 2, c = i & 3, rank = r0 + c * 8;
+                    bf16x8 high = {}, rest = {};
+                    if (of_row[r] == number && rank < l.rank) {
+                        f32x4 sum[2] = {};
+                        for (int k = 0; k < l.chunks; ++k) {
+                            const f32x4* const from = (const f32x4*)(l.low + (((int64_t)k * a.layout.num_rows + first + r) * l.rank + rank));
+                            sum[0] += from[0];
+                            sum[1] += from[1];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float v = sum[j >> 2][j & 3];
+                            high[j] = (__bf16)v;
+                            rest[j] = (__bf16)(v - (float)high[j]);
+                        }
+                    }
+                    const int key = (r >> 1) & 7;
+                    *(bf16x8*)(to_rows + r * 128 + ((c ^ key) << 4)) = high;
+                    *(bf16x8*)(to_rows + r * 128 + (((c + 4) ^ key) << 4)) = rest;
+                }
+                for (int i = threadIdx.x; i < TN * 4; i += THREADS) {
+                    const int r = i >> 2, c = i & 3, rank = r0 + c * 8;
+                    u32x4 v = {0u, 0u, 0u, 0u};
+                    if (r < num_columns && rank < l.rank) v = *(const u32x4*)(up + number * l.up_adapter + r * l.up_ld + rank * 2);
+                    const int key = (r >> 1) & 7;
+                    *(u32x4*)(to_columns + r * 128 + ((c ^ key) << 4)) = v;
+                    *(u32x4*)(to_columns + r * 128 + (((c + 4) ^ key) << 4)) = v;
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                multiply(to_columns, to_rows);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        }
+    }
+
     // Rows of the layout times the weights of their expert: out[r, c] = sum_d rows[r, d] columns[e(r)][c, d]
     __device__ __forceinline__ static void rows_kernel(const EpGemmArgs& a, int group) {
         const int row_tiles = count_row_tiles<TM>(a.layout);
@@ -389,7 +474,8 @@ struct Gemm {
         const char* const columns = a.columns + t.expert * a.columns_expert + (COLUMNS_T ? c0 * 2 : c0 * a.columns_ld);
         run(a, a.rows + t.first * a.rows_ld, columns, t.valid, t.limit, a.num_columns - (int)c0, a.depth,
             a.rows_sf + (FP8 ? t.first * a.rows_sf_row : 0), a.columns_sf + (FP8 ? t.expert * a.columns_sf_expert + c0 / 128 * a.columns_sf_row : 0),
-            a.out + (t.first * a.out_ld + c0) * OUT_ELEM);
+            a.out + (t.first * a.out_ld + c0) * OUT_ELEM, t.first,
+            LORA ? a.lora.up + t.expert * a.lora.up_expert + c0 * a.lora.up_ld : nullptr);
     }
 
     // Gradient of an expert's weights: out[e][r, c] = sum over the expert's rows d of rows[d, r] columns[d, c]
@@ -413,11 +499,110 @@ struct Gemm {
 EP_GEMM_ROWS(ep_grouped_bf16, 128, 128, 2, 2, 2, false, false, 8)
 EP_GEMM_ROWS(ep_grouped_fp8, 128, 128, 2, 2, 2, true, false, 8)
 EP_GEMM_ROWS(ep_grouped_transposed_bf16, 128, 128, 2, 2, 2, false, true, 8)
+extern "C" __global__ __launch_bounds__(256) void ep_grouped_lora_bf16(EpGemmArgs a) {
+    Gemm<128, 128, 2, 2, 2, false, false, false, false, true>::rows_kernel(a, 8);
+}
 extern "C" __global__ __launch_bounds__(256) void ep_grouped_weights_bf16(EpGemmArgs a) {
     Gemm<128, 128, 2, 2, 2, false, true, true, false>::weights_kernel(a, 8);
 }
 extern "C" __global__ __launch_bounds__(256) void ep_grouped_weights_f32(EpGemmArgs a) {
     Gemm<128, 128, 2, 2, 2, false, true, true, true>::weights_kernel(a, 8);
+}
+
+// ---- low-rank adapters: rows times the first matrix ---------------------------------------------------------
+//
+// low[chunk][r] = scale[a] * sum over the chunk's channels of down[a][e] rows[r].  A workgroup has ROWS rows of an expert, a chunk of the
+// depth, which its four waves share 128 channels at a time, and every `slots`-th of the adapters that its rows have: all rows are
+// multiplied with an adapter's matrix, and the rows that have it keep what they get.  Operands go from memory straight to
+// registers: nothing is used twice but by the neighbouring waves, out of the caches.
+template <int ROWS, int RANKS>
+__device__ __forceinline__ void lora_down_body(const EpGemmArgs& a) {
+    constexpr int NR = ROWS / 16, NK = RANKS / 16, PARTS = EP_LORA_STEP / 128;
+    __shared__ int of_row[ROWS];
+    __shared__ __attribute__((aligned(16))) float sums[4][ROWS][RANKS + 4];
+    const EpLoraArgs& l = a.lora;
+    const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
+    int at = blockIdx.x;
+    const int slot = at % l.slots;
+    at /= l.slots;
+    const int chunk = at % l.chunks, tile = at / l.chunks;
+    const RowTile t = find_row_tile<ROWS>(a.layout, tile);
+    if (t.valid <= 0) return;
+    note_adapters<ROWS>(l, t.first, t.valid, of_row, 256);
+    __syncthreads();
+    const int begin = chunk * l.chunk_depth, end = min(begin + l.chunk_depth, a.depth);
+    const char* const rows = a.rows + t.first * a.rows_ld;
+    int n = 0;
+    for (int number = next_adapter<ROWS>(of_row, -1); number != NO_ADAPTER; number = next_adapter<ROWS>(of_row, number)) {
+        if (n++ % l.slots != slot) continue;
+        const char* const down = l.down + number * l.down_adapter + t.expert * l.down_expert;
+        f32x4 acc[NR][NK];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k0 = begin + wave * 32 * PARTS; k0 < end; k0 += 128 * PARTS) {
+            u32x4 x[PARTS][NR], w[PARTS][NK];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                const int k = k0 + p * 32 + (lane >> 4) * 8;
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    const int r = i * 16 + (lane & 15);
+                    x[p][i] = r < t.valid && k < end ? *(const u32x4*)(rows + r * a.rows_ld + (int64_t)k * 2) : u32x4{0u, 0u, 0u, 0u};
+                }
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    const int r = j * 16 + (lane & 15);
+                    w[p][j] = r < l.rank && k < end ? *(const u32x4*)(down + r * l.down_ld + (int64_t)k * 2) : u32x4{0u, 0u, 0u, 0u};
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int j = 0; j < NK; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[p][j]),
+                                                                            __builtin_bit_cast(bf16x8, x[p][i]), acc[i][j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < NK; ++j) *(f32x4*)&sums[wave][i * 16 + (lane & 15)][j * 16 + (lane >> 4) * 4] = acc[i][j];
+        __syncthreads();
+        const float scale = l.scales != nullptr ? l.scales[number] : 1.0f;
+        for (int i = threadIdx.x; i < ROWS * (RANKS / 4); i += 256) {
+            const int r = i / (RANKS / 4), c = (i - r * (RANKS / 4)) * 4;
+            if (of_row[r] != number || c >= l.rank) continue;
+            const f32x4 sum = (*(const f32x4*)&sums[0][r][c] + *(const f32x4*)&sums[1][r][c]) + (*(const f32x4*)&sums[2][r][c] + *(const f32x4*)&sums[3][r][c]);
+            *(f32x4*)(l.low + (((int64_t)chunk * a.layout.num_rows + t.first + r) * l.rank + c)) = sum * scale;
+        }
+        __syncthreads();
+    }
+}
+#define EP_LORA_DOWN(ROWS, RANKS) \
+    extern "C" __global__ __launch_bounds__(256) void ep_lora_down_##ROWS##_##RANKS(EpGemmArgs a) { lora_down_body<ROWS, RANKS>(a); }
+EP_LORA_DOWN(16, 16)
+EP_LORA_DOWN(16, 32)
+EP_LORA_DOWN(16, 64)
+EP_LORA_DOWN(32, 16)
+EP_LORA_DOWN(32, 32)
+EP_LORA_DOWN(32, 64)
+
+// ---- a token's number at the rows that it was sent to --------------------------------------------------------
+
+extern "C" __global__ __launch_bounds__(256) void ep_expand_fill(EpExpandIndexArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < a.num_out) a.out[i] = -1;
+}
+extern "C" __global__ __launch_bounds__(256) void ep_expand_token_index_rows(EpExpandIndexArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int row = (int)(i / a.topk), k = (int)(i - (int64_t)row * a.topk);
+    if (row >= min(a.num_rows, a.psum_rank[a.num_ranks - 1])) return;
+    const int* const m = a.metadata + (int64_t)row * (a.topk + 2);
+    const int slot = m[k], token = m[a.topk];
+    if (slot >= 0 && slot < a.num_out && token >= 0 && token < a.num_values) a.out[slot] = a.values[token];
 }
 
 // ---- the gated activation -----------------------------------------------------------------------------

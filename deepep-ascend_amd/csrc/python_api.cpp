@@ -594,11 +594,11 @@ void on_current_device(std::initializer_list<const at::Tensor*> tensors) {
 }
 const at::Tensor* of(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 
-at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf, const OptTensor& psum,
-                          int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
+// (the result, allocated where the caller brings none)
+at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf,
+                       const OptTensor& psum, int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
     on_current_device({&x, of(x_sf), &weight, of(weight_sf), of(psum), of(out)});
     EP_PY_ASSERT(x.dim() == 2);
-    ep_grouped_linear_args_t a{};
     a.x = desc(x);
     a.x_sf = desc(x_sf);
     a.weight = expert_matrix(weight, a.weight_expert_stride);
@@ -614,8 +614,63 @@ at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::
     a.zero_rows = zero_rows;
     a.transpose_weight = transpose_weight;
     a.stream = current_stream();
+    return y;
+}
+
+at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf, const OptTensor& psum,
+                          int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
+    ep_grouped_linear_args_t a{};
+    const at::Tensor y = fill_linear(a, x, x_sf, weight, weight_sf, psum, alignment, out, zero_rows, transpose_weight);
     check(ep_grouped_linear(&a));
     return y;
+}
+
+// An adapter's matrices: [adapters, rows, columns], or [adapters, experts, rows, columns].
+ep_tensor_t adapter_matrix(const at::Tensor& t, int num_adapters, int num_experts, int64_t& adapter_stride, int64_t& expert_stride) {
+    EP_PY_ASSERT(t.dim() == 3 || t.dim() == 4);
+    EP_PY_ASSERT(t.size(0) == num_adapters && (t.dim() == 4 ? t.size(1) == num_experts : num_experts == 1));
+    ep_tensor_t d{};
+    d.data = t.data_ptr() != nullptr ? t.data_ptr() : nonnull_ptr(t);
+    d.dtype = dtype_code(t, false);
+    d.ndim = 2;
+    for (int i = 0; i < 2; ++i) {
+        d.size[i] = t.size(t.dim() - 2 + i);
+        d.stride[i] = t.stride(t.dim() - 2 + i);
+    }
+    adapter_stride = num_adapters > 1 ? t.stride(0) : 0;
+    expert_stride = t.dim() == 4 && num_experts > 1 ? t.stride(1) : 0;
+    return d;
+}
+
+at::Tensor grouped_lora_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& lora_a, const at::Tensor& lora_b,
+                               const at::Tensor& adapter_idx, const OptTensor& scales, const OptTensor& psum, int alignment, const OptTensor& out,
+                               int zero_rows) {
+    on_current_device({&lora_a, &lora_b, &adapter_idx, of(scales)});
+    ep_grouped_lora_args_t a{};
+    const at::Tensor y = fill_linear(a.linear, x, std::nullopt, weight, std::nullopt, psum, alignment, out, zero_rows, false);
+    EP_PY_ASSERT(lora_a.dim() >= 3);
+    a.num_adapters = (int)lora_a.size(0);
+    a.lora_a = adapter_matrix(lora_a, a.num_adapters, a.linear.num_experts, a.lora_a_adapter_stride, a.lora_a_expert_stride);
+    a.lora_b = adapter_matrix(lora_b, a.num_adapters, a.linear.num_experts, a.lora_b_adapter_stride, a.lora_b_expert_stride);
+    a.adapter_idx = desc(adapter_idx);
+    a.scales = desc(scales);
+    a.workspace_bytes = ep_grouped_lora_workspace_bytes(x.size(0), a.linear.num_experts, x.size(1), (int)lora_a.size(-2));
+    at::Tensor workspace;
+    if (a.workspace_bytes > 0) {
+        workspace = alloc({a.workspace_bytes}, at::kByte, x.device());
+        a.workspace = workspace.data_ptr();
+    }
+    check(ep_grouped_lora_linear(&a));
+    return y;
+}
+
+at::Tensor expand_token_index(const at::Tensor& values, const at::Tensor& src_metadata, const at::Tensor& psum_rank, int64_t num_rows) {
+    on_current_device({&values, &src_metadata, &psum_rank});
+    EP_PY_ASSERT(num_rows >= 0);
+    const at::Tensor out = alloc({num_rows}, at::kInt, values.device());
+    const ep_tensor_t v = desc(values), m = desc(src_metadata), p = desc(psum_rank), o = desc(out);
+    check(ep_expand_token_index(&v, &m, &p, &o, current_stream()));
+    return out;
 }
 
 at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, const OptTensor& psum, int num_experts, int alignment,
@@ -692,6 +747,8 @@ PYBIND11_MODULE(_native, m) {
         return py::make_tuple((int64_t)stream.id(), (int)stream.device_index(), (int)stream.unwrap().device_type());
     }, "(stream_id, device_index, device_type) of the current stream");
     m.def("grouped_linear", &grouped_linear);
+    m.def("grouped_lora_linear", &grouped_lora_linear);
+    m.def("expand_token_index", &expand_token_index);
     m.def("grouped_weight_grad", &grouped_weight_grad);
     m.def("swiglu", &swiglu);
     m.def("swiglu_grad", &swiglu_grad);

@@ -14,7 +14,8 @@ from .buffers.ep import EPBuffer, EPHandle                                      
 from ._C import (get_num_allocation_alignment, get_num_rdma_alignment,               # noqa: E402
                  get_num_tma_alignment, topk_idx_t)
 from .utils.event import EventHandle, EventOverlap                                   # noqa: E402
-from .experts import (grouped_linear, grouped_linear_grad, swiglu, swiglu_grad)      # noqa: E402
+from .experts import (expand_token_index, grouped_linear, grouped_linear_grad,        # noqa: E402
+                      grouped_lora_linear, swiglu, swiglu_grad)
 
 
 def init_jit() -> None:

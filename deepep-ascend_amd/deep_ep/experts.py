@@ -173,3 +173,36 @@ def swiglu_grad(grad: torch.Tensor, h: torch.Tensor, layout: _Layout = None, top
     """Gradients of `swiglu` without autograd: `(grad_h [rows, 2 * I] bfloat16, grad_topk_weights [rows] float32` or None `)`."""
     psum, alignment = _layout(layout)
     return _native.swiglu_grad(_rows(grad), h, topk_weights, psum, _num_experts(psum), alignment, do_zero_padding)
+
+
+def grouped_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_idx: torch.Tensor,
+                        layout: _Layout = None, *, scales: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                        do_zero_padding: bool = False) -> torch.Tensor:
+    """`grouped_linear` with low-rank adapters of many requests beside the experts' weights, or (without a layout) beside one
+    projection that all rows share: `y[m] = weight[e] @ x[m] + scales[a] * lora_b[a, e] @ (lora_a[a, e] @ x[m])` with the row's expert
+    `e` and adapter `a = adapter_idx[m]`.
+
+    Arguments:
+        x: `[rows, K]` bfloat16; weight: `[experts, N, K]` or `[N, K]` bfloat16.
+        lora_a: `[adapters, experts, R, K]` bfloat16, lora_b: `[adapters, experts, N, R]`; without the experts' dimension where there is one.
+            R is a multiple of 8 up to 64.
+        adapter_idx: `[rows]` int32; a row whose number is outside `[0, adapters)` has no adapter.  `expand_token_index` makes it from
+            the tokens' numbers.
+        scales: `[adapters]` float32 or None.
+        layout, out, do_zero_padding: as for `grouped_linear`.
+
+    The low-rank rows are held in 32 bits.  For inference: no gradients.
+    """
+    psum, alignment = _layout(layout)
+    if _wants_grad(x, weight, lora_a, lora_b, scales):
+        raise AssertionError('gradients of adapters are not implemented')
+    return _native.grouped_lora_linear(x, weight, lora_a, lora_b, adapter_idx, scales, psum, alignment, out, do_zero_padding)
+
+
+def expand_token_index(handle: EPHandle, values: torch.Tensor) -> torch.Tensor:
+    """A number of every token, such as its adapter's, at the rows that the dispatch made of it: `[num_expanded_tokens]` int32, -1 in
+    rows of no expert.  `values`: `[num_tokens]` int32; of several partitions all tokens', partition p's from
+    `p * num_max_tokens_per_rank` on."""
+    if handle.recv_src_metadata is None:
+        raise AssertionError('the handle comes from a dispatch that ran its epilogue')
+    return _native.expand_token_index(values, handle.recv_src_metadata, handle.psum_num_recv_tokens_per_rank, handle.num_expanded_tokens)

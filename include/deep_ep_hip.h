@@ -343,6 +343,30 @@ typedef struct ep_grouped_linear_args {
 /* out[m] = W[e(m)] x[m].  FP8: sums over groups of 128 channels, each scaled by x_sf[m,g] * weight_sf[e(m),n/128,g]. */
 int ep_grouped_linear(const ep_grouped_linear_args_t* args);
 
+/* Low-rank adapters of many requests beside the product: out[m] = W[e(m)] x[m] + scales[a] B[a,e(m)] (A[a,e(m)] x[m]) with
+ * a = adapter_idx[m]; a row whose number is outside [0, num_adapters) has none.  BF16; the low-rank rows are held in 32 bits. */
+typedef struct ep_grouped_lora_args {
+    ep_grouped_linear_args_t linear;
+    ep_tensor_t lora_a;                 /* [R,K] BF16 of adapter 0 and expert 0, R a multiple of 8 up to EP_LORA_MAX_RANK */
+    ep_tensor_t lora_b;                 /* [N,R] BF16 of adapter 0 and expert 0 */
+    ep_tensor_t adapter_idx;            /* [M] int32 */
+    ep_tensor_t scales;                 /* [num_adapters] fp32 (optional) */
+    int64_t lora_a_adapter_stride, lora_a_expert_stride, lora_b_adapter_stride, lora_b_expert_stride;    /* elements */
+    int32_t num_adapters, reserved;
+    void* workspace;                    /* ep_grouped_lora_workspace_bytes(M, E, K, R) bytes of the call's own */
+    int64_t workspace_bytes;
+} ep_grouped_lora_args_t;
+#define EP_LORA_MAX_RANK 64
+/* -1: sizes that the call would refuse. */
+int64_t ep_grouped_lora_workspace_bytes(int64_t num_rows, int num_experts, int64_t depth, int rank);
+int ep_grouped_lora_linear(const ep_grouped_lora_args_t* args);
+
+/* A number of every token (of its adapter, its request) at the rows that the dispatch made of it: out[slot] = values[token] for
+ * the slots of every received token, -1 elsewhere.  values [num tokens, of several partitions (partition * num_max_tokens_per_rank +
+ * token)] int32; src_metadata and psum_num_recv_tokens_per_rank are the dispatch's; out [N_exp] int32. */
+int ep_expand_token_index(const ep_tensor_t* values, const ep_tensor_t* src_metadata, const ep_tensor_t* psum_num_recv_tokens_per_rank,
+                          const ep_tensor_t* out, void* stream);
+
 typedef struct ep_grouped_weight_grad_args {
     ep_tensor_t grad;                   /* [M,N] BF16: gradient of the result */
     ep_tensor_t x;                      /* [M,K] BF16 */

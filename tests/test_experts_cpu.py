@@ -7,6 +7,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF16, FP8, I32, F32 = 1, 2, 4, 6
+ENTRIES = ('ep_grouped_linear', 'ep_grouped_lora_linear', 'ep_grouped_weight_grad', 'ep_swiglu', 'ep_swiglu_grad')
 
 
 class Tensor(ctypes.Structure):
@@ -43,11 +44,17 @@ class SwigluGrad(ctypes.Structure):
         (n, ctypes.c_int32) for n in ('num_experts', 'expert_alignment', 'zero_rows')] + [('stream', ctypes.c_void_p)]
 
 
+class Lora(ctypes.Structure):
+    _fields_ = [('linear', Linear)] + [(n, Tensor) for n in ('lora_a', 'lora_b', 'adapter_idx', 'scales')] + [
+        (n, ctypes.c_int64) for n in ('a_adapter', 'a_expert', 'b_adapter', 'b_expert')] + [
+        ('num_adapters', ctypes.c_int32), ('reserved', ctypes.c_int32), ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64)]
+
+
 @pytest.fixture(scope='module')
 def lib():
     import deep_ep
     lib = deep_ep._C._lib
-    for name in ('ep_grouped_linear', 'ep_grouped_weight_grad', 'ep_swiglu', 'ep_swiglu_grad'):
+    for name in ENTRIES:
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [ctypes.c_void_p]
     lib.ep_last_error.restype = ctypes.c_char_p
@@ -158,8 +165,53 @@ def test_swiglu_grad_refuses(lib, change):
 
 
 def test_missing_arguments_are_refused(lib):
-    for name in ('ep_grouped_linear', 'ep_grouped_weight_grad', 'ep_swiglu', 'ep_swiglu_grad'):
+    for name in ENTRIES:
         assert getattr(lib, name)(None) != 0
+    assert lib.ep_expand_token_index(None, None, None, None, None) != 0
+
+
+def lora(**changes):
+    values = dict(linear=linear(), lora_a=matrix(16, 256), lora_b=matrix(128, 16), adapter_idx=vector(64, I32), a_adapter=4 * 16 * 256,
+                  a_expert=16 * 256, b_adapter=4 * 128 * 16, b_expert=128 * 16, num_adapters=3, workspace=4096, workspace_bytes=1 << 30)
+    values.update(changes)
+    a = Lora()
+    for k, v in values.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize('change', [
+    dict(linear=linear(fp8=True)), dict(linear=linear(x=matrix(64, 128), out=matrix(64, 256), transpose_weight=1)),
+    dict(lora_a=matrix(16, 248, ld=256)), dict(lora_a=matrix(12, 256), lora_b=matrix(128, 12, ld=16)),
+    dict(lora_a=matrix(72, 256), lora_b=matrix(128, 72)), dict(lora_b=matrix(120, 16)), dict(lora_b=matrix(128, 8)),
+    dict(lora_a=matrix(16, 256, F32)), dict(num_adapters=0), dict(a_adapter=4), dict(b_expert=-8), dict(adapter_idx=vector(63, I32)),
+    dict(adapter_idx=vector(64, 5)), dict(adapter_idx=Tensor()), dict(scales=vector(2, F32)), dict(scales=vector(3, BF16)),
+    dict(workspace=None), dict(workspace=4100), dict(workspace_bytes=64 * 16 * 4 - 1)])
+def test_grouped_lora_refuses(lib, change):
+    refused(lib, 'ep_grouped_lora_linear', lora(**change))
+
+
+def test_lora_workspace(lib):
+    f = lib.ep_grouped_lora_workspace_bytes
+    f.restype, f.argtypes = ctypes.c_int64, [ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int]
+    for bad in ((-1, 1, 64, 8), (4, 0, 64, 8), (4, 1, 0, 8), (4, 1, 64, 0), (4, 1, 64, 72)):
+        assert f(*bad) == -1
+    assert f(0, 1, 64, 8) == 0
+    for rows in (1, 7, 61, 500, 3000, 100000):
+        for experts in (1, 8, 160):
+            for depth in (8, 512, 520, 7168):
+                chunks, rest = divmod(f(rows, experts, depth, 16), rows * 16 * 4)
+                assert rest == 0 and 1 <= chunks <= 16 and chunks <= -(-depth // 512)
+
+
+@pytest.mark.parametrize('change', [dict(values=vector(8, 5)), dict(metadata=matrix(8, 2, I32)), dict(metadata=vector(8, I32)), dict(psum=vector(0, I32)),
+                                    dict(psum=Tensor()), dict(out=vector(16, F32)), dict(out=vector(16, I32, stride=2))])
+def test_expand_token_index_refuses(lib, change):
+    a = {**dict(values=vector(8, I32), metadata=matrix(8, 4, I32), psum=vector(1, I32), out=vector(16, I32)), **change}
+    f = lib.ep_expand_token_index
+    f.argtypes = [ctypes.c_void_p] * 5
+    assert f(*(ctypes.addressof(a[k]) for k in ('values', 'metadata', 'psum', 'out')), None) != 0
+    assert lib.ep_last_error().decode().startswith('Assertion exception (ep_experts.cpp:')
 
 
 def test_tensors_of_the_host_are_refused():
@@ -182,5 +234,7 @@ def test_what_has_no_gradient_is_refused():
         deep_ep.grouped_linear((torch.zeros(4, 16).to(torch.float8_e4m3fn), torch.ones(4, 1, requires_grad=True)), w)
     with pytest.raises(AssertionError, match='gradients'):
         deep_ep.swiglu(x, fused_fp8_quant=True)
+    with pytest.raises(AssertionError, match='gradients'):
+        deep_ep.grouped_lora_linear(x, w, w[None], w[None], torch.zeros(4, dtype=torch.int32))
     with pytest.raises(AssertionError, match='pair'):
         deep_ep.swiglu(x.detach(), out=torch.zeros(4, 8, dtype=torch.bfloat16), fused_fp8_quant=True)

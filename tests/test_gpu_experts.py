@@ -193,3 +193,295 @@ def test_swiglu_at_the_ends_of_the_range():
     assert ((got[0] - want[0]).abs() <= want[0].abs() * 2.0 ** -7 + 1e-35).all()
     q, sf = deep_ep.swiglu(h.to(DEV), fused_fp8_quant=True)
     assert torch.isnan(q[1].float()).all() and torch.isfinite(q[0].float()).all() and torch.isfinite(sf[0]).all()
+
+
+def _lora_inputs(layout, adapters, rank, depth, columns, shared, seed=5):
+    experts = len(layout.counts)
+    x, w = U.normal(seed, layout.rows, depth), U.normal(seed + 1, experts, columns, depth, scale=depth ** -0.5)
+    a = U.normal(seed + 2, adapters, experts, rank, depth, scale=depth ** -0.5)
+    b = U.normal(seed + 3, adapters, experts, columns, rank)
+    scales = torch.rand(adapters, generator=torch.Generator().manual_seed(seed + 4)) + 0.5
+    return x, w, a, b, scales
+
+
+def _lora(x, w, a, b, scales, idx, layout):
+    """Values, and what the tolerance counts: the product's magnitudes, and the adapters' part's with both of its sums."""
+    y, size = U.linear(x, w, layout)
+    low_size = torch.zeros_like(y)
+    for e, mine in enumerate(layout.slices()):
+        for n in range(a.size(0)):
+            rows = torch.arange(layout.rows)[mine][idx[mine] == n]
+            s = 1.0 if scales is None else scales[n].double()
+            y[rows] += s * (x[rows].double() @ a[n, e].double().t()) @ b[n, e].double().t()
+            low_size[rows] += s * (x[rows].double().abs() @ a[n, e].double().abs().t()) @ b[n, e].double().abs().t()
+    return y, size, low_size
+
+
+@pytest.mark.parametrize('name', LAYOUTS)
+@pytest.mark.parametrize('adapters,rank,depth,columns', [(1, 8, 8, 8), (3, 16, 264, 136), (40, 40, 1032, 72), (7, 64, 520, 264)])
+@pytest.mark.parametrize('mixed', [False, True])
+def test_grouped_lora(name, adapters, rank, depth, columns, mixed):
+    layout = U.Layout(*LAYOUTS[name])
+    x, w, a, b, scales = _lora_inputs(layout, adapters, rank, depth, columns, False)
+    gen = torch.Generator().manual_seed(9)
+    # any order, or in runs as requests have it; numbers of no adapter on either side
+    idx = torch.randint(-1, adapters + 1, (layout.rows,), generator=gen) if mixed else \
+        torch.arange(layout.rows) * (adapters + 2) // max(1, layout.rows) - 1
+    idx = idx.to(torch.int32)
+    scales = scales if mixed else None
+    want, size, low = _lora(x, w, a, b, scales, idx, layout)
+    idx[~layout.valid] = 0
+    U.spoil(x, layout)
+    out = _sentinel(layout.rows, columns)
+    deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a), _dev(b), _dev(idx), layout.on(DEV), scales=None if scales is None else _dev(scales), out=out)
+    # the low-rank rows are sums in 32 bits too, handed on as two BF16 that keep 2^-17 of them
+    more = low * (2.0 ** -17 + (depth + rank + 16) * U.STEP_F32)
+    v = layout.valid
+    U.assert_sum(out[v.to(DEV)], want[v], size[v], depth, what=name, more=more[v])
+    _check_rows(out, layout, False, 77.0)
+
+
+@pytest.mark.parametrize('rows', [0, 1, 17, 61, 300, 2300])
+def test_lora_beside_a_shared_projection(rows):
+    layout = U.Layout([rows], 1)
+    x, w, a, b, scales = _lora_inputs(layout, 5, 16, 1024, 256, True)
+    idx = torch.randint(0, 5, (rows,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    want, size, low = _lora(x, w, a, b, scales, idx, layout)
+    y = deep_ep.grouped_lora_linear(_dev(x), _dev(w[0]), _dev(a[:, 0]), _dev(b[:, 0]), _dev(idx), scales=_dev(scales))
+    U.assert_sum(y, want, size, 1024, more=low * (2.0 ** -17 + 2048 * U.STEP_F32))
+    # without adapters it is the product alone, to the last bit
+    none = torch.full((rows,), -1, dtype=torch.int32, device=DEV)
+    assert torch.equal(deep_ep.grouped_lora_linear(_dev(x), _dev(w[0]), _dev(a[:, 0]), _dev(b[:, 0]), none), deep_ep.grouped_linear(_dev(x), _dev(w[0])))
+
+
+def test_adapters_as_views():
+    """Matrices of adapters and experts inside larger tensors, and one that all adapters share."""
+    layout = U.Layout([20, 3, 40], 8)
+    x, w, a, b, scales = _lora_inputs(layout, 4, 16, 128, 64, False)
+    idx = torch.randint(-1, 4, (layout.rows,), generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    want = deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a), _dev(b), _dev(idx), layout.on(DEV), do_zero_padding=True)
+    wide_a, wide_b = torch.zeros(3, 4, 24, 136, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 3, 64, 40, dtype=torch.bfloat16, device=DEV)
+    va, vb = wide_a.transpose(0, 1)[:, :, 8:, :128], wide_b[..., 8:24]
+    va.copy_(a), vb.copy_(b)
+    wide_x = torch.zeros(layout.rows, 256, dtype=torch.bfloat16, device=DEV)
+    vx = wide_x[:, 64:192]
+    vx.copy_(x)
+    wide_w = torch.zeros(64, 3, 128, dtype=torch.bfloat16, device=DEV)
+    vw = wide_w.transpose(0, 1)
+    vw.copy_(w)
+    got = deep_ep.grouped_lora_linear(vx, vw, va, vb, _dev(idx), layout.on(DEV), do_zero_padding=True)
+    assert torch.equal(got, want)
+    one = deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a[1:2].expand(4, -1, -1, -1).contiguous()), _dev(b), _dev(idx), layout.on(DEV), do_zero_padding=True)
+    same = deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a)[1:2].expand(4, -1, -1, -1), _dev(b), _dev(idx), layout.on(DEV), do_zero_padding=True)
+    assert torch.equal(one, same)
+
+
+def test_views_of_rows_scales_and_results():
+    layout = U.Layout([70, 0, 9], 16, 5)
+    x, w = U.quantise_rows(U.normal(1, layout.rows, 320)), U.quantise_weights(U.normal(2, 3, 136, 320))
+    want = deep_ep.grouped_linear(_dev(x), _dev(w), layout.on(DEV), do_zero_padding=True)
+    # scales by columns, as a dispatch with use_tma_aligned_col_major_sf returns them; weights' scales transposed; a slice of a wider result
+    columns = _dev(x[1]).t().contiguous().t()
+    scales = _dev(w[1]).transpose(1, 2).contiguous().transpose(1, 2)
+    wide = _sentinel(layout.rows, 200)
+    deep_ep.grouped_linear((_dev(x[0]), columns), (_dev(w[0]), scales), layout.on(DEV), out=wide[:, 32:168], do_zero_padding=True)
+    covered = (layout.valid | layout.padding).to(DEV)
+    assert torch.equal(wide[covered, 32:168], want[covered])
+    assert (wide[:, :32] == 77).all() and (wide[:, 168:] == 77).all() and (wide[~covered] == 77).all()
+    h = _dev(U.normal(3, layout.rows, 512))
+    a, (q, sf) = deep_ep.swiglu(h, layout.on(DEV), do_zero_padding=True), deep_ep.swiglu(h, layout.on(DEV), fused_fp8_quant=True, do_zero_padding=True)
+    wide_h = torch.zeros(layout.rows, 1024, dtype=torch.bfloat16, device=DEV)
+    wide_h[:, 256:768] = h
+    by_columns = torch.zeros(2, layout.rows, device=DEV).t()
+    wide_q = torch.zeros(layout.rows, 264, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    deep_ep.swiglu(wide_h[:, 256:768], layout.on(DEV), fused_fp8_quant=True, out=(wide_q[:, 8:], by_columns), do_zero_padding=True)
+    assert torch.equal(wide_q[:, 8:].float()[covered], q.float()[covered]) and torch.equal(by_columns[covered], sf[covered])
+    assert torch.equal(deep_ep.swiglu(wide_h[:, 256:768], layout.on(DEV), do_zero_padding=True)[covered], a[covered])
+
+
+def test_counts_beyond_the_tensors_stay_inside():
+    """Whatever the counts say, no row outside the tensors is touched (an expert that ends behind the last row ends with it)."""
+    x, w = _dev(U.normal(1, 40, 64)), _dev(U.normal(2, 3, 32, 64))
+    wide = _sentinel(104, 32)
+    psum = torch.tensor([30, 200, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    deep_ep.grouped_linear(x, w, (psum, 16), out=wide[32:72], do_zero_padding=True)
+    assert (wide[:32] == 77).all() and (wide[72:] == 77).all()
+    want = deep_ep.grouped_linear(x, w, (torch.tensor([30, 40, 40], dtype=torch.int32, device=DEV), 16), do_zero_padding=True)
+    assert torch.equal(wide[32:72], want)
+    deep_ep.swiglu(x, (psum, 16), out=wide[32:72])
+    assert (wide[:32] == 77).all() and (wide[72:] == 77).all()
+    negative = torch.tensor([-5, -(2 ** 31), 7], dtype=torch.int32, device=DEV)
+    deep_ep.grouped_linear(x, w, (negative, 16), out=wide[32:72])
+    deep_ep.swiglu(x, (negative, 16), out=wide[32:72])
+    deep_ep.grouped_linear_grad(_dev(U.normal(3, 40, 32)), x, w, (psum, 16))
+    assert (wide[:32] == 77).all() and (wide[72:] == 77).all()
+
+
+def test_broadcast_gradients():
+    layout = U.Layout([5, 20], 8)
+    x, w = _dev(U.normal(1, layout.rows, 64)).requires_grad_(), _dev(U.normal(2, 2, 32, 64)).requires_grad_()
+    y = deep_ep.grouped_linear(x, w, layout.on(DEV), do_zero_padding=True)
+    y.sum().backward()                                   # a gradient of one value, broadcast
+    gx, gw = deep_ep.grouped_linear_grad(torch.ones_like(y), x.detach(), w.detach(), layout.on(DEV), do_zero_padding=True)
+    assert torch.equal(x.grad, gx) and torch.equal(w.grad, gw)
+    h = _dev(U.normal(3, layout.rows, 64)).requires_grad_()
+    a = deep_ep.swiglu(h, layout.on(DEV), do_zero_padding=True)
+    a.t().contiguous().t().sum(dim=0).sum().backward()
+    assert torch.equal(h.grad, deep_ep.swiglu_grad(torch.ones_like(a), h.detach(), layout.on(DEV), do_zero_padding=True)[0])
+
+
+# ---- together, as they are used -----------------------------------------------------------------------------
+
+def _moe(tokens, hidden, inner, experts, topk, alignment, seed=0):
+    from helpers import make_routing
+    idx, weights = make_routing(tokens, experts, topk, seed=seed, masked=0.1)
+    x = U.normal(seed, tokens, hidden)
+    up, down = U.normal(seed + 1, experts, 2 * inner, hidden, scale=hidden ** -0.5), U.normal(seed + 2, experts, hidden, inner, scale=inner ** -0.5)
+    buf = deep_ep.EPBuffer(deep_ep.LocalGroup(), num_max_tokens_per_rank=tokens, hidden=hidden, num_topk=topk)
+    return x, idx, weights, up, down, buf
+
+
+def _moe_values(x, idx, weights, up, down):
+    out = torch.zeros(x.shape, dtype=torch.float64)
+    for t in range(x.size(0)):
+        for k in range(idx.size(1)):
+            e = int(idx[t, k])
+            if e >= 0:
+                h = x[t] @ up[e].t()
+                gate, u = h.chunk(2)
+                out[t] = out[t] + (gate * torch.sigmoid(gate) * u * weights[t, k]) @ down[e].t()
+    return out
+
+
+@pytest.mark.parametrize('sync', [False, True])
+@pytest.mark.parametrize('alignment', [1, 128])
+@pytest.mark.parametrize('fp8', [False, True])
+def test_dispatch_experts_combine(sync, alignment, fp8):
+    tokens, hidden, inner, experts, topk = 77, 256, 128, 9, 3
+    x, idx, weights, up, down, buf = _moe(tokens, hidden, inner, experts, topk, alignment)
+    recv, _, recv_w, handle, _ = buf.dispatch(_dev(x), topk_idx=_dev(idx), topk_weights=_dev(weights), num_experts=experts,
+                                              expert_alignment=alignment, do_expand=True, do_cpu_sync=sync, fused_fp8_quant=fp8)
+    wu, wd = (U.quantise_weights(up), U.quantise_weights(down)) if fp8 else (up, down)
+    h = deep_ep.grouped_linear(recv, _dev(wu), handle)
+    a = deep_ep.swiglu(h, handle, recv_w, fused_fp8_quant=fp8)
+    y = deep_ep.grouped_linear(a, _dev(wd), handle)
+    out, _, _ = buf.combine(y, handle)
+    wx = U.widen_rows(U.quantise_rows(x)) if fp8 else x.double()
+    want = _moe_values(wx, idx, weights.double(), U.widen_weights(wu), U.widen_weights(wd))
+    # three roundings to BF16 (h, y, out) and one of the activation; in FP8 the activation's is 2^-4 of it; relative to the values' size
+    rel = (out.cpu().double() - want).norm() / want.norm()
+    assert rel <= (2.0 ** -4 + 4 * U.HALF_BF16 if fp8 else 6 * U.HALF_BF16), rel
+
+
+def test_training_step_of_the_experts():
+    """Forward and backward through dispatch, experts and combine, against the gradients of the formula in 64 bits."""
+    tokens, hidden, inner, experts, topk = 40, 128, 64, 5, 2
+    x, idx, weights, up, down, buf = _moe(tokens, hidden, inner, experts, topk, 16)
+    grad_out = U.normal(7, tokens, hidden)
+    rx, rw, ru, rd = (t.double().requires_grad_() for t in (x, weights, up, down))
+    _moe_values(rx, idx, rw, ru, rd).backward(grad_out.double())
+    with torch.no_grad():
+        recv, _, recv_w, handle, _ = buf.dispatch(_dev(x), topk_idx=_dev(idx), topk_weights=_dev(weights), num_experts=experts,
+                                                  expert_alignment=16, do_expand=True)
+    recv, recv_w = recv.requires_grad_(), recv_w.requires_grad_()
+    du, dd = _dev(up).requires_grad_(), _dev(down).requires_grad_()
+    y = deep_ep.grouped_linear(deep_ep.swiglu(deep_ep.grouped_linear(recv, du, handle), handle, recv_w), dd, handle)
+    out, _, _ = buf.combine(y.detach(), handle)
+    grad_rows, _, _, _, _ = buf.dispatch(_dev(grad_out), handle=handle, do_expand=True)
+    y.backward(grad_rows)
+    grad_x, grad_w, _ = buf.combine(recv.grad, handle, topk_weights=recv_w.grad)
+    rel = lambda got, want: ((got.cpu().double() - want).norm() / want.norm()).item()  # noqa: E731
+    # at most six roundings to BF16 on the way to each of them
+    for got, want in ((grad_x, rx.grad), (grad_w, rw.grad), (du.grad, ru.grad), (dd.grad, rd.grad)):
+        assert rel(got, want) <= 8 * U.HALF_BF16
+
+
+def test_adapters_of_tokens_behind_a_dispatch():
+    tokens, hidden, experts, topk, adapters = 50, 128, 6, 2, 4
+    x, idx, weights, up, _, buf = _moe(tokens, hidden, 64, experts, topk, 8)
+    of_token = torch.randint(-1, adapters, (tokens,), generator=torch.Generator().manual_seed(3)).to(torch.int32)
+    a, b = U.normal(4, adapters, experts, 16, hidden, scale=hidden ** -0.5), U.normal(5, adapters, experts, 128, 16)
+    for sync in (False, True):
+        recv, _, _, handle, _ = buf.dispatch(_dev(x), topk_idx=_dev(idx), topk_weights=_dev(weights), num_experts=experts, expert_alignment=8,
+                                             do_expand=True, do_cpu_sync=sync)
+        of_row = deep_ep.expand_token_index(handle, _dev(of_token))
+        assert of_row.shape == (handle.num_expanded_tokens,)
+        slots = handle.recv_src_metadata.cpu()
+        want = torch.full((handle.num_expanded_tokens,), -1, dtype=torch.int32)
+        for row in slots[:int(handle.psum_num_recv_tokens_per_rank.cpu()[-1])]:
+            for s in row[:topk]:
+                if s >= 0:
+                    want[s] = of_token[row[topk]]
+        assert torch.equal(of_row.cpu(), want)
+        y = deep_ep.grouped_lora_linear(recv, _dev(up), _dev(a), _dev(b), of_row, handle)
+        assert y.shape == (recv.size(0), 128)
+    s, e = next((int(r[k]), int(idx[r[topk], k])) for r in slots for k in range(topk) if r[k] >= 0 and of_token[r[topk]] >= 0)
+    row, n = recv[s].cpu().double(), int(want[s])
+    value = row @ up[e].double().t() + (row @ a[n, e].double().t()) @ b[n, e].double().t()
+    assert ((y[s].cpu().double() - value).norm() / value.norm()) <= 2 * U.HALF_BF16
+
+
+def test_captured_with_a_dispatch_and_replayed():
+    """Dispatch, experts with adapters, combine in one graph, replayed over new inputs, with eager work between."""
+    tokens, hidden, inner, experts, topk = 32, 256, 128, 8, 2
+    x, idx, weights, up, down, buf = _moe(tokens, hidden, inner, experts, topk, 16)
+    up, down = _dev(up), _dev(down)
+    a, b = _dev(U.normal(4, 3, experts, 8, hidden, scale=hidden ** -0.5)), _dev(U.normal(5, 3, experts, 2 * inner, 8))
+    static = [_dev(x), _dev(idx), _dev(weights), _dev(torch.zeros(tokens, dtype=torch.int32))]
+
+    def step():
+        recv, _, recv_w, handle, _ = buf.dispatch(static[0], topk_idx=static[1], topk_weights=static[2], num_experts=experts,
+                                                  expert_alignment=16, do_expand=True, do_cpu_sync=False)
+        of_row = deep_ep.expand_token_index(handle, static[3])
+        h = deep_ep.grouped_lora_linear(recv, up, a, b, of_row, handle)
+        y = deep_ep.grouped_linear(deep_ep.swiglu(h, handle, recv_w), down, handle)
+        gx, gw = deep_ep.grouped_linear_grad(y, deep_ep.swiglu(h, handle, recv_w), down, handle, need_x=False)
+        return buf.combine(y, handle)[0], gw
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(4):
+        nx, nidx, nw, *_ = _moe(tokens, hidden, inner, experts, topk, 16, seed=10 + seed)
+        for s, v in zip(static, (nx, nidx, nw, torch.randint(-1, 3, (tokens,), generator=torch.Generator().manual_seed(seed)).to(torch.int32))):
+            s.copy_(v)
+        graph.replay()
+        got = [t.clone() for t in captured]
+        for g, w in zip(got, step()):
+            assert torch.equal(g, w)
+        torch.cuda.synchronize()
+
+
+def test_on_another_stream():
+    layout = U.Layout([300, 20], 16)
+    x, w = _dev(U.normal(1, layout.rows, 256)), _dev(U.normal(2, 2, 256, 256))
+    want = deep_ep.grouped_linear(x, w, layout.on(DEV), do_zero_padding=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf = x.detach().requires_grad_()
+        y = deep_ep.grouped_linear(leaf, w, layout.on(DEV), do_zero_padding=True)
+        y.backward(y.detach())
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y.detach(), want)
+    assert torch.equal(leaf.grad, deep_ep.grouped_linear_grad(want, x, w, layout.on(DEV), need_weight=False, do_zero_padding=True)[0])
+
+
+def test_results_do_not_change_from_run_to_run():
+    layout = U.Layout([513, 40, 7], 32)
+    x, w, a, b, scales = (_dev(t) for t in _lora_inputs(layout, 6, 16, 2048, 512, False))
+    idx = _dev(torch.randint(-1, 6, (layout.rows,), generator=torch.Generator().manual_seed(2)).to(torch.int32))
+    grad = _dev(U.normal(8, layout.rows, 512))
+
+    def once():
+        y = deep_ep.grouped_lora_linear(x, w, a, b, idx, layout.on(DEV), scales=scales, do_zero_padding=True)
+        return (y, *deep_ep.grouped_linear_grad(grad, x, w, layout.on(DEV), do_zero_padding=True))
+    first = once()
+    for _ in range(3):
+        for f, g in zip(first, once()):
+            assert torch.equal(f, g)

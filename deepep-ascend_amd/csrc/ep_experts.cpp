@@ -9,11 +9,21 @@
 
 namespace {
 
+// Tiles of the products: output rows, output columns, threads of a workgroup.
+struct Tile {
+    int rows, columns, threads;
+};
+constexpr Tile kTiles[] = {{32, 64, 256}, {64, 128, 256}, {128, 128, 512}, {256, 256, 512}};
+constexpr int kNumTiles = 4, kTile32 = 0, kTile64 = 1, kTile128 = 2, kTile256 = 3;
+constexpr int kKindBf16 = 0, kKindFp8 = 1, kKindLora = 2, kKindTransposed = 3;
+
 struct ExpertKernels {
     hipModule_t module = nullptr;
     int device = -1;
-    hipFunction_t bf16, fp8, transposed, lora, weights[2], swiglu[2], swiglu_grad;
-    hipFunction_t lora_down[2][3], expand_fill, expand_rows;
+    hipFunction_t rows[4][kNumTiles];             // [kKind*][kTiles]
+    hipFunction_t split[3], sum_splits;           // [kKind*]
+    hipFunction_t weights[2][2];                  // [BF16, float32][128 x 128, 256 x 256]
+    hipFunction_t swiglu[2], swiglu_grad, lora_down[2][3], expand_fill, expand_rows;
 };
 ExpertKernels g_k;
 std::mutex g_mutex;
@@ -68,11 +78,37 @@ EpExpertLayout layout_of(const ep_tensor_t& psum, int num_experts, int alignment
 }
 
 // Row tiles of all experts are at most this many: every expert with rows begins a tile of its own.
-int64_t row_tiles_bound(const EpExpertLayout& l, int tile) {
-    return l.num_rows / tile + std::min<int64_t>(l.num_experts, l.num_rows);
+int64_t row_tiles_bound(int64_t rows, int num_experts, int tile) {
+    return num_experts == 1 ? ceil_div(rows, tile) : rows / tile + std::min<int64_t>(num_experts, rows);
 }
 
-constexpr int kTile = 128;
+// How a product of rows is launched: its tile, and in how many parts of the depth.
+struct Plan {
+    int tile, splits, split_depth;
+};
+Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool fp8, bool transposed) {
+    // what an expert has on average, were the padding as much as it can be: the counts are known on the device only
+    const int64_t real = std::max<int64_t>(rows - (int64_t)(alignment - 1) * num_experts, std::min<int64_t>(rows, num_experts));
+    const int64_t mean = ceil_div(real, num_experts);
+    Plan p{kTile256, 1, 0};
+    if (mean <= 48) p.tile = kTile64;
+    else if (mean <= 160) p.tile = kTile128;
+    if (transposed) {
+        p.tile = std::max(p.tile, kTile128);
+        return p;
+    }
+    if (p.tile == kTile64 or rows <= 1024) {
+        const int64_t tiles = row_tiles_bound(rows, num_experts, kTiles[kTile64].rows) * ceil_div(columns, kTiles[kTile64].columns);
+        const int64_t steps = ceil_div(depth, 128);
+        if (tiles < 256) {
+            p.splits = (int)std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
+            p.split_depth = (int)(ceil_div(steps, p.splits) * 128);
+            p.splits = (int)ceil_div(depth, p.split_depth);
+            p.tile = p.splits > 1 ? kTile64 : kTile32;
+        }
+    }
+    return p;
+}
 
 }  // namespace
 
@@ -87,16 +123,23 @@ void ep_load_expert_kernels(const char* dir) {
     hipModule_t m;
     HIP_CHECK(hipModuleLoad(&m, path.c_str()));
     auto get = [&](hipFunction_t& fn, const char* name) { HIP_CHECK(hipModuleGetFunction(&fn, m, name)); };
-    get(g_k.bf16, "ep_grouped_bf16");
-    get(g_k.fp8, "ep_grouped_fp8");
-    get(g_k.transposed, "ep_grouped_transposed_bf16");
-    get(g_k.lora, "ep_grouped_lora_bf16");
+    const char* kinds[] = {"bf16", "fp8", "lora", "transposed"};
+    for (int k = 0; k < 4; ++k) {
+        for (int t = 0; t < kNumTiles; ++t) {
+            if (k == kKindTransposed and t < kTile128) continue;
+            get(g_k.rows[k][t], format("ep_grouped_%s_%dx%d", kinds[k], kTiles[t].rows, kTiles[t].columns).c_str());
+        }
+    }
+    for (int k = 0; k < 3; ++k) get(g_k.split[k], format("ep_grouped_split_%s", kinds[k]).c_str());
+    get(g_k.sum_splits, "ep_sum_splits");
     for (int i = 0; i < 2; ++i)
         for (int j = 0; j < 3; ++j) get(g_k.lora_down[i][j], format("ep_lora_down_%d_%d", 16 << i, 16 << j).c_str());
     get(g_k.expand_fill, "ep_expand_fill");
     get(g_k.expand_rows, "ep_expand_token_index_rows");
-    get(g_k.weights[0], "ep_grouped_weights_bf16");
-    get(g_k.weights[1], "ep_grouped_weights_f32");
+    const char* outs[] = {"bf16", "f32"};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j)
+            get(g_k.weights[i][j], format("ep_grouped_weights_%s_%dx%d", outs[i], 128 << j, 128 << j).c_str());
     get(g_k.swiglu[0], "ep_swiglu_bf16");
     get(g_k.swiglu[1], "ep_swiglu_fp8");
     get(g_k.swiglu_grad, "ep_swiglu_gradients");
@@ -108,6 +151,8 @@ extern "C" {
 // The arguments of a product of rows, checked.
 static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
     const ep_tensor_t &x = args->x, &w = args->weight, &out = args->out;
+    EP_HOST_ASSERT(args->workspace_bytes >= 0 and (args->workspace != nullptr or args->workspace_bytes == 0));
+    EP_HOST_ASSERT(((uintptr_t)args->workspace & 15) == 0);
     EP_HOST_ASSERT(row_major(x) and addressable(x));
     EP_HOST_ASSERT(row_major(w) and addressable(w) and w.dtype == x.dtype);
     const bool fp8 = x.dtype == EP_DTYPE_FP8_E4M3, transposed = args->transpose_weight != 0;
@@ -147,8 +192,41 @@ static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
         g.columns_sf_col = wsf.stride[1];
         g.columns_sf_expert = args->weight_sf_expert_stride;
     }
-    g.column_tiles = (int)ceil_div(columns, kTile);
     return g;
+}
+
+// The launches of a product of rows; `workspace`: where the parts of a split depth go, if there is room.
+static void launch_rows(EpGemmArgs& g, int kind, void* workspace, int64_t workspace_bytes, void* stream) {
+    const EpExpertLayout& l = g.layout;
+    Plan p = plan_rows(l.num_rows, l.num_experts, l.alignment, g.depth, g.num_columns, kind == kKindFp8, kind == kKindTransposed);
+    const ExpertKernels& k = kernels();
+    if (p.splits > 1 and (int64_t)p.splits * l.num_rows * g.num_columns * 4 > workspace_bytes) p = Plan{kTile32, 1, 0};
+    const Tile& t = kTiles[p.tile];
+    g.column_tiles = (int)ceil_div(g.num_columns, t.columns);
+    g.splits = p.splits;
+    g.split_depth = p.split_depth;
+    g.partial = (float*)workspace;
+    const int64_t row_tiles = row_tiles_bound(l.num_rows, l.num_experts, t.rows);
+    EP_HOST_ASSERT(row_tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles * p.splits));
+    launch(p.splits > 1 ? k.split[kind] : k.rows[kind][p.tile], align_up(row_tiles * g.column_tiles * p.splits, 8), t.threads, stream, g);
+    if (p.splits == 1) return;
+    EpSumSplitsArgs s{};
+    s.layout = l;
+    s.partial = g.partial;
+    s.out = g.out;
+    s.out_ld = g.out_ld;
+    s.splits = p.splits;
+    s.num_columns = g.num_columns;
+    launch(k.sum_splits, ceil_div((int64_t)l.num_rows * ceil_div(g.num_columns, 512), 4), 256, stream, s);
+}
+
+int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns,
+                                          int dtype) {
+    if (num_rows <= 0 or num_rows > INT32_MAX or num_experts <= 0 or expert_alignment <= 0 or depth <= 0 or depth > INT32_MAX / 2 or num_columns <= 0 or
+        num_columns > INT32_MAX / 2)
+        return 0;
+    const Plan p = plan_rows(num_rows, num_experts, expert_alignment, depth, num_columns, dtype == EP_DTYPE_FP8_E4M3, false);
+    return p.splits > 1 ? (int64_t)p.splits * num_rows * num_columns * 4 : 0;
 }
 
 int ep_grouped_linear(const ep_grouped_linear_args_t* args) {
@@ -156,9 +234,8 @@ int ep_grouped_linear(const ep_grouped_linear_args_t* args) {
         EP_HOST_ASSERT(args != nullptr);
         EpGemmArgs g = linear_args(args);
         if (g.layout.num_rows == 0) return;
-        const ExpertKernels& k = kernels();
-        launch(args->x.dtype == EP_DTYPE_FP8_E4M3 ? k.fp8 : args->transpose_weight ? k.transposed : k.bf16,
-               align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256, args->stream, g);
+        launch_rows(g, args->x.dtype == EP_DTYPE_FP8_E4M3 ? kKindFp8 : args->transpose_weight ? kKindTransposed : kKindBf16, args->workspace,
+                    args->workspace_bytes, args->stream);
     });
 }
 
@@ -224,10 +301,10 @@ int ep_grouped_lora_linear(const ep_grouped_lora_args_t* args) {
         l.chunk_depth = plan.chunk_depth;
         l.slots = plan.slots;
         const ExpertKernels& k = kernels();
-        const int64_t tiles = row_tiles_bound(g.layout, plan.rows);
+        const int64_t tiles = row_tiles_bound(g.layout.num_rows, g.layout.num_experts, plan.rows);
         launch(k.lora_down[plan.rows == 16 ? 0 : 1][rank <= 16 ? 0 : rank <= 32 ? 1 : 2], tiles * plan.chunks * plan.slots, 256,
                args->linear.stream, g);
-        launch(k.lora, align_up(row_tiles_bound(g.layout, kTile) * g.column_tiles, 8), 256, args->linear.stream, g);
+        launch_rows(g, kKindLora, args->linear.workspace, args->linear.workspace_bytes, args->linear.stream);
     });
 }
 
@@ -281,12 +358,15 @@ int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
         g.out_expert = args->out_expert_stride;
         g.num_columns = (int)x.size[1];
         g.num_out_rows = (int)grad.size[1];
-        g.column_tiles = (int)ceil_div(g.num_columns, kTile);
-        g.row_tiles = (int)ceil_div(g.num_out_rows, kTile);
+        // (tiles of 256 x 256 as soon as they fill the chip)
+        const bool large = (int64_t)g.layout.num_experts * ceil_div(g.num_columns, 256) * ceil_div(g.num_out_rows, 256) >= 256;
+        const int tile = large ? 256 : 128;
+        g.column_tiles = (int)ceil_div(g.num_columns, tile);
+        g.row_tiles = (int)ceil_div(g.num_out_rows, tile);
         g.accumulate = args->accumulate != 0;
         const int64_t tiles = (int64_t)g.layout.num_experts * g.row_tiles;
-        EP_HOST_ASSERT(tiles <= INT32_MAX / std::max(1, g.column_tiles));
-        launch(kernels().weights[f32 ? 1 : 0], align_up(tiles * g.column_tiles, 8), 256, args->stream, g);
+        EP_HOST_ASSERT(tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles));
+        launch(kernels().weights[f32 ? 1 : 0][large ? 1 : 0], align_up(tiles * g.column_tiles, 8), 512, args->stream, g);
     });
 }
 

@@ -14,6 +14,7 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -102,6 +103,24 @@ __device__ __forceinline__ RowTile find_row_tile(const EpExpertLayout& l, int ti
     return t;
 }
 
+// 0: not a row to write, 1: one to write zeros into, 2: a row of an expert
+__device__ __forceinline__ int kind_of_row(const EpExpertLayout& l, int row) {
+    if (l.psum == nullptr) return 2;
+    // experts that end at or before the row, and where the last of them ends
+    int before = 0, end = 0;
+    for (int e0 = 0; e0 < l.num_experts; e0 += WAVE) {
+        const int e = e0 + lane_id();
+        const int p = e < l.num_experts ? l.psum[e] : 0x7fffffff;
+        const int n = __popcll(__ballot(p <= row));
+        if (n > 0) end = __builtin_amdgcn_readlane(p, n - 1);
+        before += n;
+        if (n < WAVE) break;
+    }
+    const int start = align_up(max(end, 0), l.alignment);
+    if (row < start) return l.zero_rows != EP_ZERO_NONE ? 1 : 0;
+    return before < l.num_experts ? 2 : l.zero_rows == EP_ZERO_ALL ? 1 : 0;
+}
+
 // Workgroup -> tile.  Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes one stretch of the tiles, and
 // within a stretch GROUP row tiles go through the column tiles together, so that what runs at once on an XCD reads few panels.
 __device__ __forceinline__ bool tile_of_block(int row_tiles, int column_tiles, int group, int& row, int& column) {
@@ -183,39 +202,37 @@ struct TileFetch {
     }
     __device__ __forceinline__ static int piece(int i, int wave) { return (wave + i * WAVES) % PIECES; }
 
-    // step `s` of the depth into the LDS at `to` (behind the last step: zeros)
-    __device__ __forceinline__ void fetch(int s, unsigned to, int wave) const {
-        if (!TRANSPOSED) {
-            const int left = depth_bytes - s * 128;
-            const i32x4 buffer = buffer_of(base + (int64_t)s * 128, left > 0 && bytes > 0 ? bytes - s * 128 : 0u);
-            if (left >= 128) {
-#pragma unroll
-                for (int i = 0; i < MINE; ++i) fetch16(to + piece(i, wave) * 1024, from[i], buffer);
-            } else {
-#pragma unroll
-                for (int i = 0; i < MINE; ++i) fetch16(to + piece(i, wave) * 1024, chunk * 16 < left ? from[i] : OUTSIDE, buffer);
-            }
-        } else {
+    // Step `s` of the depth (behind the last step: zeros): its buffer, and its fetches.  Steps come in order.
+    __device__ __forceinline__ i32x4 step(int s) {
+        if (TRANSPOSED) {
             const int rows = min(depth - s * 64, 64);
-            const i32x4 buffer = buffer_of(base + (int64_t)s * 64 * ld, rows > 0 ? (unsigned)((rows - 1) * ld) + bytes : 0u);
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) fetch16(to + piece(i, wave) * 1024, from[i], buffer);
+            return buffer_of(base + (int64_t)s * 64 * ld, rows > 0 ? (unsigned)((rows - 1) * ld) + bytes : 0u);
         }
+        const int left = depth_bytes - s * 128;
+        if (left < 128) {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) from[i] = chunk * 16 < left ? from[i] : OUTSIDE;
+        }
+        return buffer_of(base + (int64_t)s * 128, left > 0 && bytes > 0 ? bytes - s * 128 : 0u);
     }
+    __device__ __forceinline__ void fetch(i32x4 buffer, int i, unsigned to, int wave) const { fetch16(to + piece(i, wave) * 1024, from[i], buffer); }
 };
 
-// The 16 rows from `first` on of a direct tile, 16 bytes a lane: row lane % 16, chunk half * 4 + lane / 16.
-__device__ __forceinline__ u32x4 direct_fragment(const char* tile, int first, int half) {
-    const int lane = lane_id(), r = lane & 15;
-    return *(const u32x4*)(tile + (first + r) * 128 + (((half * 4 + (lane >> 4)) ^ (r >> 1)) << 4));
+// What a lane gives a matrix instruction over MT rows (or columns) of an operand, 16 bytes at a time: of row lane % MT, chunk
+// q * (64 / MT) + lane / MT of the step's eight.
+template <int MT>
+__device__ __forceinline__ u32x4 direct_fragment(const char* tile, int first, int q) {
+    const int lane = lane_id(), r = lane % MT;
+    return *(const u32x4*)(tile + (first + r) * 128 + (((q * (WAVE / MT) + lane / MT) ^ ((r >> 1) & 7)) << 4));
 }
-// The 16 columns from `first` on of a transposed tile, rows half * 32 + lane / 16 * 8 + (0 .. 7) of them: two transposing reads, each of
-// which hands the lanes of a group of 16 the columns of the four 32-byte row pieces that the group reads.
-template <int T>
-__device__ __forceinline__ u32x4 transposed_fragment(const char* tile, int first, int half) {
-    const int lane = lane_id(), j = (lane >> 2) & 3, b = lane >> 4;
-    const int granule = (first >> 4) ^ (j | (b & 1) << 2);
-    const lds_byte* at = (const lds_byte*)(tile + (half * 32 + b * 8 + j) * (T * 2) + granule * 32 + (lane & 3) * 8);
+// The same of a transposed tile, columns from `first` on: two transposing reads, each of which hands the lanes of a group of 16 the columns
+// of the four 32-byte row pieces that the group reads.
+template <int MT, int T>
+__device__ __forceinline__ u32x4 transposed_fragment(const char* tile, int first, int q) {
+    const int lane = lane_id(), j = (lane >> 2) & 3;
+    const int row = (q * (WAVE / MT) + lane / MT) * 8 + j, column = first + (lane % MT & 16);
+    const int granule = (column >> 4) ^ (j | ((lane / MT) & 1) << 2);
+    const lds_byte* at = (const lds_byte*)(tile + row * (T * 2) + granule * 32 + (lane & 3) * 8);
     typedef __attribute__((address_space(3))) i16x4* quad;
     union {
         i16x4 q[2];
@@ -226,16 +243,43 @@ __device__ __forceinline__ u32x4 transposed_fragment(const char* tile, int first
     return f.v;
 }
 
-template <bool TRANSPOSED, int T>
-__device__ __forceinline__ u32x4 fragment(const char* tile, int first, int half) {
-    if (TRANSPOSED) return transposed_fragment<T>(tile, first, half);
-    return direct_fragment(tile, first, half);
+template <bool TRANSPOSED, int MT, int T>
+__device__ __forceinline__ u32x4 fragment(const char* tile, int first, int q) {
+    if (TRANSPOSED) return transposed_fragment<MT, T>(tile, first, q);
+    return direct_fragment<MT>(tile, first, q);
 }
 
-union Fragment8 {
+template <int MT>
+struct Sums;
+template <>
+struct Sums<16> {
+    typedef f32x4 type;
+};
+template <>
+struct Sums<32> {
+    typedef f32x16 type;
+};
+// MT x MT sums += BF16 columns x BF16 rows
+__device__ __forceinline__ f32x4 multiply_add(u32x4 c, u32x4 r, f32x4 sums) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, r), sums, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 multiply_add(u32x4 c, u32x4 r, f32x16 sums) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, r), sums, 0, 0, 0);
+}
+// ... e4m3: two chunks of each
+union Chunks {
     u32x4 half[2];
     i32x8 v;
 };
+__device__ __forceinline__ f32x4 multiply_add_fp8(const Chunks& c, const Chunks& r, f32x4 sums) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(c.v, r.v, sums, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 multiply_add_fp8(const Chunks& c, const Chunks& r, f32x16 sums) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(c.v, r.v, sums, 0, 0, 0, 0, 0, 0);
+}
+
+// The compiler keeps what is in front of this in front.
+#define KEEP_ORDER() __builtin_amdgcn_sched_barrier(0)
 
 // ---- low-rank adapters: numbers of a tile ------------------------------------------------------------------
 
@@ -269,24 +313,28 @@ __device__ __forceinline__ void note_adapters(const EpLoraArgs& l, int first, in
 //
 // One workgroup computes TM x TN of the output, WR x WC waves a part each, in 32 bits.  The matrix instruction's first operand is
 // the output's columns, its second the rows: a lane then holds four neighbouring columns of one row.
-template <int TM, int TN, int WR, int WC, int STAGES, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false>
+template <int TM, int TN, int WR, int WC, int MT, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false>
 struct Gemm {
-    static constexpr int WAVES = WR * WC, FM = TM / WR, FN = TN / WC, NR = FM / 16, NC = FN / 16;
+    static constexpr int WAVES = WR * WC, FM = TM / WR, FN = TN / WC, NR = FM / MT, NC = FN / MT;
+    static constexpr int Q = MT / 8, HQ = Q / 2;      // fragments of a step and of half of one
     static constexpr int COLUMNS_BYTES = TN * 128, ROWS_BYTES = TM * 128, SF_BYTES = FP8 ? (TM < WAVE ? WAVE : TM) * 4 : 0;
-    static constexpr int STAGE_BYTES = COLUMNS_BYTES + ROWS_BYTES + SF_BYTES;
-    static constexpr int OUT_ELEM = OUT32 ? 4 : 2, OUT_ROW = FN * OUT_ELEM + 16, OUT_BYTES = WAVES * 16 * OUT_ROW;
+    static constexpr int STAGES_BYTES = SC * COLUMNS_BYTES + SR * (ROWS_BYTES + SF_BYTES), ROWS_AT = SC * COLUMNS_BYTES, SF_AT = ROWS_AT + SR * ROWS_BYTES;
+    static_assert(SC == SR || SC == SR + 1, "stages of the two operands");
+    static constexpr int OUT_ELEM = OUT32 ? 4 : 2, OUT_ROW = FN * OUT_ELEM + 16, OUT_BYTES = WAVES * MT * OUT_ROW;
     static constexpr int BLOCKS = (TN + 127) / 128, TABLE = EP_EXPERT_MAX_DEPTH_FP8 / 128;
     static constexpr int TABLE_BYTES = FP8 ? BLOCKS * TABLE * 4 : 0;
-    static constexpr int LDS_BYTES = STAGES * STAGE_BYTES > OUT_BYTES ? STAGES * STAGE_BYTES : OUT_BYTES;
+    static constexpr int LDS_BYTES = STAGES_BYTES > OUT_BYTES ? STAGES_BYTES : OUT_BYTES;
     typedef TileFetch<TN, WAVES, COLUMNS_T> ColumnsFetch;
     typedef TileFetch<TM, WAVES, ROWS_T> RowsFetch;
     static constexpr int FETCHES = ColumnsFetch::MINE + RowsFetch::MINE + (FP8 ? 1 : 0);       // of a wave and step
     static constexpr int STEP = FP8 ? 128 : 64;
+    // fetches that a wave may have left when the rows and columns of a step have to be there, `ahead` steps before the newest
+    static constexpr int pending(int ahead) { return ahead * FETCHES + (SC > SR ? ColumnsFetch::MINE : 0); }
 
     // rows .. rows + valid: what is computed, up to limit zeros are written; columns from column on
     __device__ __forceinline__ static void run(const EpGemmArgs& a, const char* rows, const char* columns, int valid, int limit,
                                                int num_columns, int depth, const float* rows_sf, const float* columns_sf, char* out,
-                                               int first = 0, const char* up = nullptr) {
+                                               int64_t out_ld, int first = 0, const char* up = nullptr) {
         __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];
         __shared__ float table[FP8 ? BLOCKS * TABLE : 1];
         __shared__ int adapters[LORA ? TM : 1];
@@ -295,11 +343,12 @@ struct Gemm {
         const unsigned lds0 = (unsigned)(size_t)(lds_byte*)lds;
         const int steps = valid > 0 ? ceil_div(depth, STEP) : 0;
 
-        f32x4 acc[NR][NC];
+        typedef typename Sums<MT>::type sums_t;
+        sums_t acc[NR][NC];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int j = 0; j < NC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NC; ++j) acc[i][j] = sums_t{};
 
         ColumnsFetch cf;
         RowsFetch rf;
@@ -317,93 +366,254 @@ struct Gemm {
                 if (b * 128 < num_columns) table[b * TABLE + g] = columns_sf[b * a.columns_sf_row + g * a.columns_sf_col];
             }
         }
-        auto fetch = [&](int s, int stage) {
-            const unsigned to = lds0 + stage * STAGE_BYTES;
-            cf.fetch(s, to, wave);
-            rf.fetch(s, to + COLUMNS_BYTES, wave);
-            if (FP8) {
-                const i32x4 buffer = buffer_of((const char*)(rows_sf + s * a.rows_sf_col), s < steps ? sf_bytes : 0u);
-                fetch4(to + COLUMNS_BYTES + ROWS_BYTES + (wave % SF_PIECES) * 256, sf_from, buffer);
-            }
+        // What a step leaves free is filled at once: with the rows SR steps on (and their scales), then with the columns SC steps on.
+        struct Fetches {
+            i32x4 columns, rows, sf;
+            unsigned to_columns, to_rows, to_sf;
         };
+        auto begin_fetch = [&](int s_rows, int slot_rows, int s_columns, int slot_columns) {
+            Fetches f;
+            f.rows = rf.step(s_rows);
+            f.columns = cf.step(s_columns);
+            if (FP8) f.sf = buffer_of((const char*)(rows_sf + s_rows * a.rows_sf_col), s_rows < steps ? sf_bytes : 0u);
+            f.to_columns = lds0 + slot_columns * COLUMNS_BYTES;
+            f.to_rows = lds0 + ROWS_AT + slot_rows * ROWS_BYTES;
+            f.to_sf = lds0 + SF_AT + slot_rows * SF_BYTES + (wave % SF_PIECES) * 256;
+            return f;
+        };
+        constexpr int OF_ROWS = RowsFetch::MINE + (FP8 ? 1 : 0);
+        auto fetch_one = [&](const Fetches& f, int i) {
+            if (i < RowsFetch::MINE) rf.fetch(f.rows, i, f.to_rows, wave);
+            else if (i < OF_ROWS) fetch4(f.to_sf, sf_from, f.sf);
+            else cf.fetch(f.columns, i - OF_ROWS, f.to_columns, wave);
+        };
+        auto fetch_all = [&](const Fetches& f, int from) {
+#pragma unroll
+            for (int i = 0; i < FETCHES; ++i)
+                if (i >= from) fetch_one(f, i);
+        };
+        int slot_rows = 0, slot_columns = 0;
+        auto next = [](int slot, int of) { return slot == of - 1 ? 0 : slot + 1; };
 
-        auto multiply = [&](const char* at, const char* at_rows) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                u32x4 c[NC], r[NR];
-#pragma unroll
-                for (int j = 0; j < NC; ++j) c[j] = fragment<COLUMNS_T, TN>(at, first_column + j * 16, half);
-#pragma unroll
-                for (int i = 0; i < NR; ++i) r[i] = fragment<ROWS_T, TM>(at_rows, first_row + i * 16, half);
-#pragma unroll
-                for (int i = 0; i < NR; ++i)
-#pragma unroll
-                    for (int j = 0; j < NC; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c[j]), __builtin_bit_cast(bf16x8, r[i]),
-                                                                           acc[i][j], 0, 0, 0);
-            }
+        // BF16: half a step is READS fragments and PRODUCTS matrix instructions.  While half a step is multiplied, the other half's
+        // fragments are read, and the step after next is fetched, one instruction at a time between the products.
+        constexpr int READS = HQ * (NC + NR), PRODUCTS = HQ * NC * NR;
+        constexpr int READ_SPAN = (PRODUCTS * 5 + 7) / 8;
+        auto read_one = [&](u32x4 (&c)[HQ][NC], u32x4 (&r)[HQ][NR], int slot_rows, int slot_columns, int half, int i) {
+            const int q = i / (NC + NR), k = i - q * (NC + NR);
+            if (k < NC) c[q][k] = fragment<COLUMNS_T, MT, TN>(lds + slot_columns * COLUMNS_BYTES, first_column + k * MT, half * HQ + q);
+            else r[q][k - NC] = fragment<ROWS_T, MT, TM>(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + (k - NC) * MT, half * HQ + q);
+        };
+        auto multiply_one = [&](const u32x4 (&c)[HQ][NC], const u32x4 (&r)[HQ][NR], int at) {
+            const int q = at / (NR * NC), i = at / NC % NR, j = at % NC;
+            acc[i][j] = multiply_add(c[q][j], r[q][i], acc[i][j]);
         };
 
         if (steps > 0) {
+            if (SC > SR) fetch_all(begin_fetch(0, 0, 0, 0), OF_ROWS);
 #pragma unroll
-            for (int s = 0; s < STAGES - 1; ++s) fetch(s, s);
+            for (int s = 0; s < SR - 1; ++s) fetch_all(begin_fetch(s, s, s + SC - SR, s + SC - SR), 0);
         }
-        if (LORA) add_adapters(a, lds + (STAGES - 1) * STAGE_BYTES, adapters, first, valid, num_columns, up, multiply);
-        int stage = 0;
-        for (int s = 0; s < steps; ++s) {
-            wait_and_meet<(STAGES - 2) * FETCHES>();
-            fetch(s + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-            const char* const at = lds + stage * STAGE_BYTES;
-            const char* const at_rows = at + COLUMNS_BYTES;
-            if (!FP8) {
-                multiply(at, at_rows);
-            } else {
-                // a step is one group of channels: its products are summed by themselves, then scaled
-                const float* const scales = (const float*)(at_rows + ROWS_BYTES);
-                const float of_columns = table[first_column / 128 * TABLE + s];
-                Fragment8 c[NC];
+        if (LORA && up != nullptr) {
+            add_adapters(a, lds + (SC - 1) * COLUMNS_BYTES, lds + ROWS_AT + (SR - 1) * ROWS_BYTES, adapters, first, valid, num_columns, up, [&] {
+                u32x4 c[HQ][NC], r[HQ][NR];
 #pragma unroll
-                for (int j = 0; j < NC; ++j)
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) c[j].half[half] = direct_fragment(at, first_column + j * 16, half);
+                    for (int i = 0; i < READS; ++i) read_one(c, r, SR - 1, SC - 1, half, i);
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    Fragment8 r;
-                    r.half[0] = direct_fragment(at_rows, first_row + i * 16, 0);
-                    r.half[1] = direct_fragment(at_rows, first_row + i * 16, 1);
-                    const float scale = scales[first_row + i * 16 + (lane & 15)] * of_columns;
+                    for (int i = 0; i < PRODUCTS; ++i) multiply_one(c, r, i);
+                }
+            });
+        }
+        if (steps > 0 && !(FP8 && NR >= 4)) fetch_all(begin_fetch(SR - 1, SR - 1, SC - 1, SC - 1), 0);
+        if constexpr (!FP8) {
+            u32x4 c[2][HQ][NC], r[2][HQ][NR];
+            // a wave whose rows do not exist only fetches: the other wave of its SIMD has the matrix unit to itself
+            const bool active = first_row < valid;
+            if (steps > 0) {
+                wait_and_meet<pending(SR - 1)>();
 #pragma unroll
-                    for (int j = 0; j < NC; ++j) {
-                        const f32x4 sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(c[j].v, r.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                for (int i = 0; i < READS; ++i) read_one(c[0], r[0], 0, 0, 0, i);
+            }
+            for (int s = 0; s < steps; ++s) {
+                if (active) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(sum[k], scale, acc[i][j][k]);
+                    for (int p = 0; p < PRODUCTS; ++p) {
+                        // (early: they have arrived before the wave waits for the others)
+#pragma unroll
+                        for (int i = 0; i < READS; ++i)
+                            if (i * READ_SPAN / READS == p) read_one(c[1], r[1], slot_rows, slot_columns, 1, i);
+                        multiply_one(c[0], r[0], p);
+                        KEEP_ORDER();
                     }
                 }
+                const Fetches f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
+                slot_rows = next(slot_rows, SR);
+                slot_columns = next(slot_columns, SC);
+                KEEP_ORDER();
+                wait_and_meet<pending(SR - 2)>();
+                KEEP_ORDER();
+                if (active) {
+#pragma unroll
+                    for (int p = 0; p < PRODUCTS; ++p) {
+#pragma unroll
+                        for (int i = 0; i < FETCHES; ++i)
+                            if (i * PRODUCTS / FETCHES == p) fetch_one(f, i);
+#pragma unroll
+                        for (int i = 0; i < READS; ++i)
+                            if (i * PRODUCTS / READS == p) read_one(c[0], r[0], slot_rows, slot_columns, 0, i);
+                        multiply_one(c[1], r[1], p);
+                        KEEP_ORDER();
+                    }
+                } else {
+                    fetch_all(f, 0);
+                }
             }
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        } else {
+            // FP8: a step is one group of channels, whose products are summed by themselves, then scaled.
+            const float* const of_block = &table[first_column / 128 * TABLE];
+            auto read_columns = [&](Chunks (&c)[HQ], int slot_columns, int j) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) c[q / 2].half[q % 2] = direct_fragment<MT>(lds + slot_columns * COLUMNS_BYTES, first_column + j * MT, q);
+            };
+            auto read_row = [&](Chunks (&r)[HQ], float& scale, int slot_rows, int i) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) r[q / 2].half[q % 2] = direct_fragment<MT>(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + i * MT, q);
+                scale = ((const float*)(lds + SF_AT + slot_rows * SF_BYTES))[first_row + i * MT + lane % MT];
+            };
+            auto multiply = [&](const Chunks (&c)[HQ], const Chunks (&r)[HQ]) {
+                sums_t sum = {};
+#pragma unroll
+                for (int q = 0; q < HQ; ++q) sum = multiply_add_fp8(c[q], r[q], sum);
+                return sum;
+            };
+            auto add_scaled = [&](sums_t& to, const sums_t& sum, float scale) {
+#pragma unroll
+                for (int k = 0; k < MT * MT / WAVE; ++k) to[k] = __builtin_fmaf(sum[k], scale, to[k]);
+            };
+            if constexpr (NR >= 4) {
+                // Rows of fragments are read two ahead; behind the last of them the waves meet, and while the last two rows are multiplied the
+                // next step's first fragments are read.  The step after next is fetched meanwhile and in the next step's first rows.  Sums
+                // are scaled DEPTH products behind.
+                static_assert(NC >= 2, "a row's scale is needed until its last sum is scaled");
+                constexpr int DEPTH = NC < 4 ? NC : 4, LAST = (NR - 2) * NC;
+                const bool active = first_row < valid;
+                constexpr int SPREAD = 2 * NC + (LAST < 2 * NC ? LAST : 2 * NC);
+                auto fetch_at = [&](const Fetches& f, int place) {
+#pragma unroll
+                    for (int i = 0; i < FETCHES; ++i)
+                        if (i * SPREAD / FETCHES == place) fetch_one(f, i);
+                };
+                // (of a step's fetches those in front of the next step's first row)
+                constexpr int AT_ONCE = (2 * NC * FETCHES + SPREAD - 1) / SPREAD;
+                Chunks c[NC][HQ], r[4][HQ];
+                float scales[4];
+                static_assert(SC == SR, "what is pending below");
+                Fetches f;
+                if (steps > 0) {
+                    f = begin_fetch(SR - 1, SR - 1, SC - 1, SC - 1);
+#pragma unroll
+                    for (int i = 0; i < AT_ONCE; ++i) fetch_one(f, i);
+                    if (!active) fetch_all(f, AT_ONCE);
+                    wait_and_meet<(SR - 2) * FETCHES + AT_ONCE>();
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) read_columns(c[j], 0, j);
+                    read_row(r[0], scales[0], 0, 0);
+                    read_row(r[1], scales[1], 0, 1);
+                }
+                for (int s = 0; s < steps; ++s) {
+                    const float of_columns = of_block[s];
+                    sums_t sums[DEPTH];
+                    // product p: of row i and column j; the last two rows column by column, so that the columns' fragments are free one by one
+                    auto row_of = [](int p) { return p < LAST ? p / NC : NR - 2 + (p - LAST) % 2; };
+                    auto column_of = [](int p) { return p < LAST ? p % NC : (p - LAST) / 2; };
+                    auto scale_one = [&](int p) {
+                        if (p >= 0) add_scaled(acc[row_of(p)][column_of(p)], sums[p % DEPTH], scales[row_of(p) % 4] * of_columns);
+                    };
+                    if (active) {
+#pragma unroll
+                        for (int p = 0; p < LAST; ++p) {
+                            fetch_at(f, p + 2 * NC);
+                            if (p % NC == 0 && p / NC + 2 < NR) read_row(r[(p / NC + 2) % 4], scales[(p / NC + 2) % 4], slot_rows, p / NC + 2);
+                            scale_one(p - DEPTH);
+                            sums[p % DEPTH] = multiply(c[column_of(p)], r[row_of(p) % 4]);
+                            KEEP_ORDER();
+                        }
+                    }
+                    f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
+                    slot_rows = next(slot_rows, SR);
+                    slot_columns = next(slot_columns, SC);
+                    KEEP_ORDER();
+                    wait_and_meet<pending(SR - 2)>();
+                    KEEP_ORDER();
+                    if (active) {
+#pragma unroll
+                        for (int p = LAST; p < NR * NC; ++p) {
+                            fetch_at(f, p - LAST);
+                            scale_one(p - DEPTH);
+                            sums[p % DEPTH] = multiply(c[column_of(p)], r[row_of(p) % 4]);
+                            if ((p - LAST) % 2 == 1) read_columns(c[column_of(p)], slot_columns, column_of(p));
+                            if (p == LAST + 1) read_row(r[0], scales[0], slot_rows, 0);
+                            if (p == LAST + 3) read_row(r[1], scales[1], slot_rows, 1);
+                            KEEP_ORDER();
+                        }
+#pragma unroll
+                        for (int p = NR * NC - DEPTH; p < NR * NC; ++p) scale_one(p);
+                    } else {
+                        fetch_all(f, 0);
+                    }
+                }
+            } else {
+                int free_rows = 0, free_columns = 0;
+                for (int s = 0; s < steps; ++s) {
+                    wait_and_meet<pending(SR - 2)>();
+                    if (s > 0) fetch_all(begin_fetch(s - 1 + SR, free_rows, s - 1 + SC, free_columns), 0);
+                    const float of_columns = of_block[s];
+                    Chunks c[NC][HQ];
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) read_columns(c[j], slot_columns, j);
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) {
+                        Chunks r[HQ];
+                        float scale;
+                        read_row(r, scale, slot_rows, i);
+#pragma unroll
+                        for (int j = 0; j < NC; ++j) add_scaled(acc[i][j], multiply(c[j], r), scale * of_columns);
+                    }
+                    free_rows = slot_rows, free_columns = slot_columns;
+                    slot_rows = next(slot_rows, SR);
+                    slot_columns = next(slot_columns, SC);
+                }
+            }
         }
         wait_and_meet<0>();      // (the last fetches, of zeros, land in LDS too)
 
-        // 16 rows of a wave's part at a time through LDS, to leave as whole lines
-        char* const mine = lds + wave * 16 * OUT_ROW;
+        // MT rows of a wave's part at a time through LDS, to leave as whole lines
+        char* const mine = lds + wave * MT * OUT_ROW;
         constexpr int LANES = FN * OUT_ELEM / 16, PASS = WAVE / LANES;      // lanes of a row, rows of a store
         const int piece = lane % LANES, column = first_column + piece * (16 / OUT_ELEM);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                char* const to = mine + (lane & 15) * OUT_ROW + (j * 16 + (lane >> 4) * 4) * OUT_ELEM;
-                if (OUT32) *(f32x4*)to = acc[i][j];
-                else *(bf16x4*)to = __builtin_convertvector(acc[i][j], bf16x4);
+#pragma unroll
+                for (int g = 0; g < MT * MT / WAVE / 4; ++g) {
+                    // four neighbouring columns of row lane % MT
+                    const f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    char* const to = mine + lane % MT * OUT_ROW + (j * MT + g * (WAVE / MT * 4) + lane / MT * 4) * OUT_ELEM;
+                    if (OUT32) *(f32x4*)to = v;
+                    else *(bf16x4*)to = __builtin_convertvector(v, bf16x4);
+                }
             }
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (int p = 0; p < 16; p += PASS) {
-                const int r16 = p + lane / LANES, r = first_row + i * 16 + r16;
-                if (r16 >= 16 || r >= limit || column >= num_columns) continue;
-                u32x4 v = *(const u32x4*)(mine + r16 * OUT_ROW + piece * 16);
+            for (int p = 0; p < MT; p += PASS) {
+                const int in = p + lane / LANES, r = first_row + i * MT + in;
+                if (in >= MT || r >= limit || column >= num_columns) continue;
+                u32x4 v = *(const u32x4*)(mine + in * OUT_ROW + piece * 16);
                 if (r >= valid) v = u32x4{0u, 0u, 0u, 0u};
-                u32x4* const to = (u32x4*)(out + ((int64_t)r * a.out_ld + column) * OUT_ELEM);
+                u32x4* const to = (u32x4*)(out + (r * out_ld + column) * OUT_ELEM);
                 if (OUT32 && a.accumulate) {
                     const f32x4 sum = *(const f32x4*)to + __builtin_bit_cast(f32x4, v);
                     v = __builtin_bit_cast(u32x4, sum);
@@ -418,12 +628,10 @@ struct Gemm {
     // every adapter that rows of the tile have, 32 ranks at a time, a step of 64 channels.  The low-rank rows are sums in 32 bits; they
     // go in as two BF16, the rounded value and the rest, against the same column of `up` twice, which keeps 2^-17 of them.
     template <typename Multiply>
-    __device__ __forceinline__ static void add_adapters(const EpGemmArgs& a, char* stage, int* of_row, int first, int valid, int num_columns,
+    __device__ __forceinline__ static void add_adapters(const EpGemmArgs& a, char* to_columns, char* to_rows, int* of_row, int first, int valid, int num_columns,
                                                         const char* up, Multiply multiply) {
         constexpr int THREADS = WAVES * WAVE;
         const EpLoraArgs& l = a.lora;
-        char* const to_columns = stage;
-        char* const to_rows = stage + COLUMNS_BYTES;
         note_adapters<TM>(l, first, valid, of_row, THREADS);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         for (int number = next_adapter<TM>(of_row, -1); number != NO_ADAPTER; number = next_adapter<TM>(of_row, number)) {
@@ -458,24 +666,39 @@ struct Gemm {
                     *(u32x4*)(to_columns + r * 128 + (((c + 4) ^ key) << 4)) = v;
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                multiply(to_columns, to_rows);
+                multiply();
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
         }
     }
 
-    // Rows of the layout times the weights of their expert: out[r, c] = sum_d rows[r, d] columns[e(r)][c, d]
+    // Rows of the layout times the weights of their expert: out[r, c] = sum_d rows[r, d] columns[e(r)][c, d].  SPLIT: of a part of
+    // the depth, in 32 bits; ep_sum_splits adds the parts.
+    template <bool SPLIT>
     __device__ __forceinline__ static void rows_kernel(const EpGemmArgs& a, int group) {
         const int row_tiles = count_row_tiles<TM>(a.layout);
-        int row, column;
-        if (!tile_of_block(row_tiles, a.column_tiles, group, row, column)) return;
+        int row, column, part = 0;
+        if (!tile_of_block(row_tiles, SPLIT ? a.column_tiles * a.splits : a.column_tiles, group, row, column)) return;
         const RowTile t = find_row_tile<TM>(a.layout, row);
-        const int64_t c0 = (int64_t)column * TN;
-        const char* const columns = a.columns + t.expert * a.columns_expert + (COLUMNS_T ? c0 * 2 : c0 * a.columns_ld);
-        run(a, a.rows + t.first * a.rows_ld, columns, t.valid, t.limit, a.num_columns - (int)c0, a.depth,
-            a.rows_sf + (FP8 ? t.first * a.rows_sf_row : 0), a.columns_sf + (FP8 ? t.expert * a.columns_sf_expert + c0 / 128 * a.columns_sf_row : 0),
-            a.out + (t.first * a.out_ld + c0) * OUT_ELEM, t.first,
-            LORA ? a.lora.up + t.expert * a.lora.up_expert + c0 * a.lora.up_ld : nullptr);
+        int64_t d0 = 0;
+        int depth = a.depth, limit = t.limit;
+        char* out = a.out;
+        if (SPLIT) {
+            part = column % a.splits;
+            column /= a.splits;
+            d0 = (int64_t)part * a.split_depth;
+            depth = min(a.split_depth, depth - (int)d0);
+            limit = t.valid;
+            out = (char*)(a.partial + (int64_t)part * a.layout.num_rows * a.num_columns);
+        }
+        const int64_t c0 = (int64_t)column * TN, out_ld = SPLIT ? a.num_columns : a.out_ld;
+        const char* const columns = a.columns + t.expert * a.columns_expert +
+                                    (COLUMNS_T ? c0 * 2 + d0 * a.columns_ld : c0 * a.columns_ld + d0 * (FP8 ? 1 : 2));
+        run(a, a.rows + t.first * a.rows_ld + d0 * (FP8 ? 1 : 2), columns, t.valid, limit, a.num_columns - (int)c0, depth,
+            a.rows_sf + (FP8 ? t.first * a.rows_sf_row + d0 / 128 * a.rows_sf_col : 0),
+            a.columns_sf + (FP8 ? t.expert * a.columns_sf_expert + c0 / 128 * a.columns_sf_row + d0 / 128 * a.columns_sf_col : 0),
+            out + (t.first * out_ld + c0) * OUT_ELEM, out_ld, t.first,
+            LORA && part == 0 ? a.lora.up + t.expert * a.lora.up_expert + c0 * a.lora.up_ld : nullptr);
     }
 
     // Gradient of an expert's weights: out[e][r, c] = sum over the expert's rows d of rows[d, r] columns[d, c]
@@ -488,26 +711,47 @@ struct Gemm {
         const int64_t start = uniform(in.start);
         const int out_rows = min(a.num_out_rows - r0, TM);
         run(a, a.rows + start * a.rows_ld + (int64_t)r0 * 2, a.columns + start * a.columns_ld + (int64_t)c0 * 2, out_rows, out_rows,
-            a.num_columns - c0, count, nullptr, nullptr, a.out + (e * a.out_expert + (int64_t)r0 * a.out_ld + c0) * OUT_ELEM);
+            a.num_columns - c0, count, nullptr, nullptr, a.out + (e * a.out_expert + (int64_t)r0 * a.out_ld + c0) * OUT_ELEM, a.out_ld);
     }
 };
 
-#define EP_GEMM_ROWS(NAME, TM, TN, WR, WC, STAGES, FP8, COLUMNS_T, GROUP)                                             \
+#define EP_GEMM_ROWS(NAME, TM, TN, WR, WC, MT, SR, SC, FP8, COLUMNS_T, GROUP)                                         \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, STAGES, FP8, COLUMNS_T, false, false>::rows_kernel(a, GROUP);                             \
+        Gemm<TM, TN, WR, WC, MT, SR, SC, FP8, COLUMNS_T, false, false>::rows_kernel<false>(a, GROUP);                 \
     }
-EP_GEMM_ROWS(ep_grouped_bf16, 128, 128, 2, 2, 2, false, false, 8)
-EP_GEMM_ROWS(ep_grouped_fp8, 128, 128, 2, 2, 2, true, false, 8)
-EP_GEMM_ROWS(ep_grouped_transposed_bf16, 128, 128, 2, 2, 2, false, true, 8)
-extern "C" __global__ __launch_bounds__(256) void ep_grouped_lora_bf16(EpGemmArgs a) {
-    Gemm<128, 128, 2, 2, 2, false, false, false, false, true>::rows_kernel(a, 8);
-}
-extern "C" __global__ __launch_bounds__(256) void ep_grouped_weights_bf16(EpGemmArgs a) {
-    Gemm<128, 128, 2, 2, 2, false, true, true, false>::weights_kernel(a, 8);
-}
-extern "C" __global__ __launch_bounds__(256) void ep_grouped_weights_f32(EpGemmArgs a) {
-    Gemm<128, 128, 2, 2, 2, false, true, true, true>::weights_kernel(a, 8);
-}
+#define EP_GEMM_SPLIT(NAME, TM, TN, WR, WC, MT, SR, SC, FP8, LORA, GROUP)                                             \
+    extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
+        Gemm<TM, TN, WR, WC, MT, SR, SC, FP8, false, false, true, LORA>::rows_kernel<true>(a, GROUP);                 \
+    }
+#define EP_GEMM_LORA(NAME, TM, TN, WR, WC, MT, SR, SC, GROUP)                                                         \
+    extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
+        Gemm<TM, TN, WR, WC, MT, SR, SC, false, false, false, false, true>::rows_kernel<false>(a, GROUP);             \
+    }
+#define EP_GEMM_WEIGHTS(NAME, TM, TN, WR, WC, MT, SR, SC, OUT32, GROUP)                                               \
+    extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
+        Gemm<TM, TN, WR, WC, MT, SR, SC, false, true, true, OUT32>::weights_kernel(a, GROUP);                         \
+    }
+EP_GEMM_ROWS(ep_grouped_bf16_32x64, 32, 64, 1, 4, 16, 4, 4, false, false, 4)
+EP_GEMM_ROWS(ep_grouped_bf16_64x128, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
+EP_GEMM_ROWS(ep_grouped_bf16_128x128, 128, 128, 2, 4, 16, 3, 3, false, false, 4)
+EP_GEMM_ROWS(ep_grouped_bf16_256x256, 256, 256, 4, 2, 16, 2, 3, false, false, 8)
+EP_GEMM_ROWS(ep_grouped_fp8_32x64, 32, 64, 1, 4, 16, 4, 4, true, false, 4)
+EP_GEMM_ROWS(ep_grouped_fp8_64x128, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
+EP_GEMM_ROWS(ep_grouped_fp8_128x128, 128, 128, 2, 4, 16, 3, 3, true, false, 4)
+EP_GEMM_ROWS(ep_grouped_fp8_256x256, 256, 256, 2, 4, 16, 2, 2, true, false, 8)
+EP_GEMM_ROWS(ep_grouped_transposed_128x128, 128, 128, 2, 4, 16, 3, 3, false, true, 4)
+EP_GEMM_ROWS(ep_grouped_transposed_256x256, 256, 256, 2, 4, 16, 2, 3, false, true, 8)
+EP_GEMM_SPLIT(ep_grouped_split_bf16, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
+EP_GEMM_SPLIT(ep_grouped_split_fp8, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
+EP_GEMM_SPLIT(ep_grouped_split_lora, 64, 128, 2, 2, 16, 3, 3, false, true, 1)
+EP_GEMM_LORA(ep_grouped_lora_32x64, 32, 64, 1, 4, 16, 4, 4, 4)
+EP_GEMM_LORA(ep_grouped_lora_64x128, 64, 128, 2, 2, 16, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_128x128, 128, 128, 2, 4, 16, 3, 3, 4)
+EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 16, 2, 2, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 3, 3, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 16, 2, 3, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 3, 3, true, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 16, 2, 3, true, 8)
 
 // ---- low-rank adapters: rows times the first matrix ---------------------------------------------------------
 //
@@ -605,6 +849,30 @@ extern "C" __global__ __launch_bounds__(256) void ep_expand_token_index_rows(EpE
     if (slot >= 0 && slot < a.num_out && token >= 0 && token < a.num_values) a.out[slot] = a.values[token];
 }
 
+// ---- parts of a depth, added -----------------------------------------------------------------------------
+
+// A lane has eight columns of a row.
+extern "C" __global__ __launch_bounds__(256) void ep_sum_splits(EpSumSplitsArgs a) {
+    const int vectors = a.num_columns >> 3, per_row = ceil_div(vectors, WAVE);
+    const int64_t task = (int64_t)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
+    const int row = uniform((int)(task / per_row)), v = (int)(task - (int64_t)row * per_row) * WAVE + lane_id();
+    if (row >= a.layout.num_rows) return;
+    const int kind = kind_of_row(a.layout, row);
+    if (kind == 0 || v >= vectors) return;
+    f32x4 sum[2] = {};
+    if (kind == 2) {
+        for (int s = 0; s < a.splits; ++s) {
+            const f32x4* const from = (const f32x4*)(a.partial + ((int64_t)s * a.layout.num_rows + row) * a.num_columns) + 2 * v;
+            sum[0] += from[0];
+            sum[1] += from[1];
+        }
+    }
+    bf16x8 out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = (__bf16)sum[i >> 2][i & 3];
+    *((bf16x8*)(a.out + row * a.out_ld * 2) + v) = out;
+}
+
 // ---- the gated activation -----------------------------------------------------------------------------
 //
 // out = silu(gate) * up * weight, a lane eight channels, a wave 512 of a row.
@@ -633,24 +901,6 @@ __device__ __forceinline__ unsigned row16_umax(unsigned x) {
     return x;
 }
 
-// 0: not a row to write, 1: one to write zeros into, 2: a row of an expert
-__device__ __forceinline__ int kind_of_row(const EpExpertLayout& l, int row) {
-    if (l.psum == nullptr) return 2;
-    // experts that end at or before the row, and where the last of them ends
-    int before = 0, end = 0;
-    for (int e0 = 0; e0 < l.num_experts; e0 += WAVE) {
-        const int e = e0 + lane_id();
-        const int p = e < l.num_experts ? l.psum[e] : 0x7fffffff;
-        const int n = __popcll(__ballot(p <= row));
-        if (n > 0) end = __builtin_amdgcn_readlane(p, n - 1);
-        before += n;
-        if (n < WAVE) break;
-    }
-    const int start = align_up(max(end, 0), l.alignment);
-    if (row < start) return l.zero_rows != EP_ZERO_NONE ? 1 : 0;
-    return before < l.num_experts ? 2 : l.zero_rows == EP_ZERO_ALL ? 1 : 0;
-}
-
 template <bool FP8>
 __device__ __forceinline__ void swiglu_body(const EpSwigluArgs& a) {
     const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
@@ -675,7 +925,7 @@ __device__ __forceinline__ void swiglu_body(const EpSwigluArgs& a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) out[i] = gate[i] * sigmoid(gate[i]) * up[i] * weight;
         }
-        if (!FP8) {
+        if constexpr (!FP8) {
             if (live) ((u32x4*)(a.out + (int64_t)row * a.out_ld * 2))[v] = round_bf16(out);
             continue;
         }

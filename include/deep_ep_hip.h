@@ -338,8 +338,12 @@ typedef struct ep_grouped_linear_args {
     int64_t weight_expert_stride, weight_sf_expert_stride;      /* elements */
     int32_t num_experts, expert_alignment, zero_rows;
     int32_t transpose_weight;           /* the product with the transposed weights (gradient of the rows), BF16 */
+    void* workspace;                    /* of the call's own, or NULL: with ep_grouped_linear_workspace_bytes bytes a product of few */
+    int64_t workspace_bytes;            /* tiles is split over its depth */
     void* stream;
 } ep_grouped_linear_args_t;
+int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns,
+                                          int dtype);
 /* out[m] = W[e(m)] x[m].  FP8: sums over groups of 128 channels, each scaled by x_sf[m,g] * weight_sf[e(m),n/128,g]. */
 int ep_grouped_linear(const ep_grouped_linear_args_t* args);
 

@@ -26,7 +26,8 @@ def vector(n, dtype, at=4096, stride=1):
 class Linear(ctypes.Structure):
     _fields_ = [(n, Tensor) for n in ('x', 'x_sf', 'weight', 'weight_sf', 'psum', 'out')] + [
         ('weight_expert_stride', ctypes.c_int64), ('weight_sf_expert_stride', ctypes.c_int64)] + [
-        (n, ctypes.c_int32) for n in ('num_experts', 'expert_alignment', 'zero_rows', 'transpose_weight')] + [('stream', ctypes.c_void_p)]
+        (n, ctypes.c_int32) for n in ('num_experts', 'expert_alignment', 'zero_rows', 'transpose_weight')] + [
+        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64), ('stream', ctypes.c_void_p)]
 
 
 class WeightGrad(ctypes.Structure):
@@ -105,6 +106,9 @@ LINEAR = {
     'too many rows': dict(x=matrix(2 ** 31, 256), out=matrix(2 ** 31, 128)),
     'rows of many megabytes': dict(x=matrix(64, 256, ld=2 ** 22)),
     'no rows tensor': dict(x=Tensor()),
+    'a workspace of no address': dict(workspace_bytes=16),
+    'a workspace off 16 bytes': dict(workspace=4104, workspace_bytes=16),
+    'a workspace of less than nothing': dict(workspace=4096, workspace_bytes=-1),
 }
 LINEAR_FP8 = {
     'no scales': dict(x_sf=Tensor()),

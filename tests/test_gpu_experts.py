@@ -97,6 +97,71 @@ def test_grouped_linear_gradients(name, depth, columns):
     U.assert_sum(total, want_w, size_w, most, half=2.0 ** -24, what='float32')
 
 
+# mean rows of an expert on both sides of the lines between tiles, tails of every size in them
+@pytest.mark.parametrize('counts', [[700, 0, 190, 513], [257, 383, 128, 64, 1], [160, 161, 90], [40, 47, 48, 49, 16], [5000]])
+@pytest.mark.parametrize('depth,columns', [(16, 520), (1008, 776), (2048, 256)])
+@pytest.mark.parametrize('kind', ['bf16', 'fp8', 'lora', 'gradients'])
+def test_every_tile(counts, depth, columns, kind):
+    layout = U.Layout(counts, 16)
+    experts = len(counts)
+    x, w = U.normal(1, layout.rows, depth), U.normal(2, experts, columns, depth, scale=depth ** -0.5)
+    v = layout.valid
+    if kind == 'gradients':
+        grad = U.normal(3, layout.rows, columns)
+        gx, gw = deep_ep.grouped_linear_grad(_dev(grad), _dev(x), _dev(w), layout.on(DEV))
+        want, size = U.linear(grad, w.transpose(1, 2), layout)
+        U.assert_sum(gx[v.to(DEV)], want[v], size[v], columns, what='rows')
+        U.assert_sum(gw, *U.weight_grad(grad, x, layout), max(counts), what='weights')
+        return
+    if kind == 'lora':
+        a, b = U.normal(4, 5, experts, 24, depth, scale=depth ** -0.5), U.normal(5, 5, experts, columns, 24)
+        idx = (torch.arange(layout.rows) // 37 % 7 - 1).to(torch.int32)
+        want, size, low = _lora(x, w, a, b, None, idx, layout)
+        y = deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a), _dev(b), _dev(idx), layout.on(DEV))
+        U.assert_sum(y[v.to(DEV)], want[v], size[v], depth, more=(low * (2.0 ** -17 + (depth + 40) * U.STEP_F32))[v])
+        return
+    more = torch.zeros((layout.rows, 1))
+    if kind == 'fp8':
+        x, w = U.quantise_rows(x), U.quantise_weights(w)
+        more = U.fp8_error(x, w, layout)
+    want, size = U.linear(x, w, layout)
+    y = deep_ep.grouped_linear(_dev(x), _dev(w), layout.on(DEV))
+    U.assert_sum(y[v.to(DEV)], want[v], size[v], depth, more=more[v])
+
+
+@pytest.mark.parametrize('counts,alignment', [([1], 1), ([61], 1), ([0, 130, 3], 16), ([9, 0, 0, 2, 30, 1, 1, 5], 8)])
+@pytest.mark.parametrize('depth,columns', [(1536, 136), (7168, 512), (7120, 264)])
+@pytest.mark.parametrize('kind', ['bf16', 'fp8', 'lora'])
+def test_depth_in_parts(counts, alignment, depth, columns, kind):
+    """Few tiles: the depth is split, the parts are added in a launch of their own."""
+    layout = U.Layout(counts, alignment, tail=3)
+    experts = len(counts)
+    assert deep_ep._C._lib.ep_grouped_linear_workspace_bytes(layout.rows, experts, alignment, deep_ep._C.ctypes.c_int64(depth),
+                                                             deep_ep._C.ctypes.c_int64(columns), 2 if kind == 'fp8' else 1) > 0
+    x, w = U.normal(1, layout.rows, depth), U.normal(2, experts, columns, depth, scale=depth ** -0.5)
+    a, b = U.normal(4, 3, experts, 8, depth, scale=depth ** -0.5), U.normal(5, 3, experts, columns, 8)
+    idx = (torch.arange(layout.rows) % 4 - 1).to(torch.int32)
+    v = layout.valid
+    more = torch.zeros((layout.rows, 1))
+    if kind == 'fp8':
+        x, w = U.quantise_rows(x), U.quantise_weights(w)
+        more = U.fp8_error(x, w, layout)
+    if kind == 'lora':
+        want, size, low = _lora(x, w, a, b, None, idx, layout)
+        more = low * (2.0 ** -17 + (depth + 40) * U.STEP_F32)
+    else:
+        want, size = U.linear(x, w, layout)
+    U.spoil(x[1] if kind == 'fp8' else x, layout)
+    for zeroed in (False, True):
+        out = _sentinel(layout.rows, columns)
+        if kind == 'lora':
+            deep_ep.grouped_lora_linear(_dev(x), _dev(w), _dev(a), _dev(b), _dev(idx), layout.on(DEV), out=out, do_zero_padding=zeroed)
+        else:
+            deep_ep.grouped_linear(_dev(x), _dev(w), layout.on(DEV), out=out, do_zero_padding=zeroed)
+        U.assert_sum(out[v.to(DEV)], want[v], size[v], depth, more=more[v])
+        _check_rows(out, layout, zeroed, 77.0)
+
+
 def test_gradients_agree_with_differences():
     """Along a direction, in 64 bits on the CPU: what the formulas of the gradients are held to is the derivative of the forward formula."""
     layout = U.Layout([3, 0, 6], 4)

@@ -21,7 +21,9 @@ struct EpLoraArgs {
     const float* scales;          // [num_adapters] or nullptr
     float* low;                   // [chunks, rows, rank]: sums over the chunks of the depth
     int num_adapters, rank, chunks;
-    int chunk_depth, slots;       // the launch in front: channels of a chunk, workgroups that share a tile's adapters
+    int chunk_depth, slots;       // of what makes them: channels of a chunk, workgroups that share a tile's adapters,
+    int blocks;                   // and workgroups in all
+    int together;                 // adapters that are multiplied at once where rows are many
 };
 
 // out[r, c] = sum_d rows[r, d] columns[c, d] over a tile of output rows and output columns.
@@ -39,17 +41,10 @@ struct EpGemmArgs {
     int num_out_rows;             // weight gradient: rows of the output of one expert
     int column_tiles, row_tiles;  // (row_tiles: weight gradient)
     int accumulate;               // weight gradient in 32 bits: added to what is there
+    int few_rows;                 // weight gradient: experts have few rows on average
     int splits, split_depth;      // the depth in so many parts (of split_depth channels), sums of each in `partial`
     float* partial;               // [splits, rows, num_columns]
     EpLoraArgs lora;
-};
-
-struct EpSumSplitsArgs {
-    EpExpertLayout layout;
-    const float* partial;         // [splits, rows, columns]
-    char* out;
-    int64_t out_ld;               // elements
-    int splits, num_columns;
 };
 
 struct EpExpandIndexArgs {

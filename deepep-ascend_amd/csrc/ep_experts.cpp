@@ -13,17 +13,17 @@ namespace {
 struct Tile {
     int rows, columns, threads;
 };
-constexpr Tile kTiles[] = {{32, 64, 256}, {64, 128, 256}, {128, 128, 512}, {256, 256, 512}};
-constexpr int kNumTiles = 4, kTile32 = 0, kTile64 = 1, kTile128 = 2, kTile256 = 3;
+constexpr Tile kTiles[] = {{32, 64, 256}, {64, 128, 256}, {64, 256, 512}, {128, 256, 512}, {256, 256, 512}};
+constexpr int kNumTiles = 5, kTile32 = 0, kTile64 = 1, kTile64Wide = 2, kTile128 = 3, kTile256 = 4;
 constexpr int kKindBf16 = 0, kKindFp8 = 1, kKindLora = 2, kKindTransposed = 3;
 
 struct ExpertKernels {
     hipModule_t module = nullptr;
     int device = -1;
     hipFunction_t rows[4][kNumTiles];             // [kKind*][kTiles]
-    hipFunction_t split[3], sum_splits;           // [kKind*]
+    hipFunction_t split[2], split_lora[3], sum_splits, sum_splits_lora;
     hipFunction_t weights[2][2];                  // [BF16, float32][128 x 128, 256 x 256]
-    hipFunction_t swiglu[2], swiglu_grad, lora_down[2][3], expand_fill, expand_rows;
+    hipFunction_t swiglu[2], swiglu_grad, lora_down[3], lora_down_rows, expand_fill, expand_rows;
 };
 ExpertKernels g_k;
 std::mutex g_mutex;
@@ -82,26 +82,25 @@ int64_t row_tiles_bound(int64_t rows, int num_experts, int tile) {
     return num_experts == 1 ? ceil_div(rows, tile) : rows / tile + std::min<int64_t>(num_experts, rows);
 }
 
+// Rows of an expert on average, were the padding as much as it can be: the counts are known on the device only.
+int64_t mean_rows(int64_t rows, int num_experts, int alignment) {
+    return ceil_div(std::max<int64_t>(rows - (int64_t)(alignment - 1) * num_experts, std::min<int64_t>(rows, num_experts)), num_experts);
+}
+
 // How a product of rows is launched: its tile, and in how many parts of the depth.
 struct Plan {
     int tile, splits, split_depth;
 };
-Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool fp8, bool transposed) {
-    // what an expert has on average, were the padding as much as it can be: the counts are known on the device only
-    const int64_t real = std::max<int64_t>(rows - (int64_t)(alignment - 1) * num_experts, std::min<int64_t>(rows, num_experts));
-    const int64_t mean = ceil_div(real, num_experts);
-    Plan p{kTile256, 1, 0};
-    if (mean <= 48) p.tile = kTile64;
-    else if (mean <= 160) p.tile = kTile128;
-    if (transposed) {
-        p.tile = std::max(p.tile, kTile128);
-        return p;
-    }
+Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool transposed) {
+    const int64_t mean = mean_rows(rows, num_experts, alignment);
+    const auto tiles = [&](int t) { return row_tiles_bound(rows, num_experts, kTiles[t].rows) * ceil_div(columns, kTiles[t].columns); };
+    Plan p{mean <= 64 ? kTile128 : kTile256, 1, 0};
+    if (transposed) return p;
+    if (mean <= 40) p.tile = tiles(kTile64Wide) <= 256 ? kTile64 : kTile64Wide;
     if (p.tile == kTile64 or rows <= 1024) {
-        const int64_t tiles = row_tiles_bound(rows, num_experts, kTiles[kTile64].rows) * ceil_div(columns, kTiles[kTile64].columns);
-        const int64_t steps = ceil_div(depth, 128);
-        if (tiles < 256) {
-            p.splits = (int)std::clamp<int64_t>(512 / std::max<int64_t>(tiles, 1), 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
+        const int64_t steps = ceil_div(depth, 128), few = tiles(kTile64);
+        if (few < 256) {
+            p.splits = (int)std::clamp<int64_t>(512 / few, 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
             p.split_depth = (int)(ceil_div(steps, p.splits) * 128);
             p.splits = (int)ceil_div(depth, p.split_depth);
             p.tile = p.splits > 1 ? kTile64 : kTile32;
@@ -130,10 +129,12 @@ void ep_load_expert_kernels(const char* dir) {
             get(g_k.rows[k][t], format("ep_grouped_%s_%dx%d", kinds[k], kTiles[t].rows, kTiles[t].columns).c_str());
         }
     }
-    for (int k = 0; k < 3; ++k) get(g_k.split[k], format("ep_grouped_split_%s", kinds[k]).c_str());
+    for (int k = 0; k < 2; ++k) get(g_k.split[k], format("ep_grouped_split_%s", kinds[k]).c_str());
+    for (int i = 0; i < 3; ++i) get(g_k.split_lora[i], format("ep_grouped_split_lora_%d", 16 << i).c_str());
     get(g_k.sum_splits, "ep_sum_splits");
-    for (int i = 0; i < 2; ++i)
-        for (int j = 0; j < 3; ++j) get(g_k.lora_down[i][j], format("ep_lora_down_%d_%d", 16 << i, 16 << j).c_str());
+    get(g_k.sum_splits_lora, "ep_sum_splits_lora");
+    for (int i = 0; i < 3; ++i) get(g_k.lora_down[i], format("ep_lora_down_16_%d", 16 << i).c_str());
+    get(g_k.lora_down_rows, "ep_lora_down_rows");
     get(g_k.expand_fill, "ep_expand_fill");
     get(g_k.expand_rows, "ep_expand_token_index_rows");
     const char* outs[] = {"bf16", "f32"};
@@ -147,6 +148,22 @@ void ep_load_expert_kernels(const char* dir) {
 }
 
 extern "C" {
+
+// How the rows times the adapters' first matrices are split: rows of a workgroup's tile, chunks of the depth, workgroups that share the
+// adapters of a tile.
+struct LoraPlan {
+    int rows, chunks, chunk_depth, slots;
+};
+static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
+    LoraPlan p{};
+    p.rows = rows <= 2048 ? 16 : 64;
+    const int64_t tiles = std::max<int64_t>(1, row_tiles_bound(rows, num_experts, p.rows));
+    p.slots = p.rows == 16 ? (int)std::clamp<int64_t>(ceil_div(512, tiles), 1, std::min<int64_t>(p.rows, std::max<int64_t>(rows, 1))) : 1;
+    const int64_t steps = ceil_div(depth, EP_LORA_STEP), chunks = std::clamp<int64_t>(ceil_div(512, tiles * p.slots), 1, std::min<int64_t>(steps, 16));
+    p.chunk_depth = (int)(ceil_div(steps, chunks) * EP_LORA_STEP);
+    p.chunks = (int)ceil_div(depth, p.chunk_depth);
+    return p;
+}
 
 // The arguments of a product of rows, checked.
 static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
@@ -196,9 +213,9 @@ static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
 }
 
 // The launches of a product of rows; `workspace`: where the parts of a split depth go, if there is room.
-static void launch_rows(EpGemmArgs& g, int kind, void* workspace, int64_t workspace_bytes, void* stream) {
+static void launch_rows(EpGemmArgs& g, int kind, const LoraPlan* lora, void* workspace, int64_t workspace_bytes, void* stream) {
     const EpExpertLayout& l = g.layout;
-    Plan p = plan_rows(l.num_rows, l.num_experts, l.alignment, g.depth, g.num_columns, kind == kKindFp8, kind == kKindTransposed);
+    Plan p = plan_rows(l.num_rows, l.num_experts, l.alignment, g.depth, g.num_columns, kind == kKindTransposed);
     const ExpertKernels& k = kernels();
     if (p.splits > 1 and (int64_t)p.splits * l.num_rows * g.num_columns * 4 > workspace_bytes) p = Plan{kTile32, 1, 0};
     const Tile& t = kTiles[p.tile];
@@ -208,24 +225,27 @@ static void launch_rows(EpGemmArgs& g, int kind, void* workspace, int64_t worksp
     g.partial = (float*)workspace;
     const int64_t row_tiles = row_tiles_bound(l.num_rows, l.num_experts, t.rows);
     EP_HOST_ASSERT(row_tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles * p.splits));
-    launch(p.splits > 1 ? k.split[kind] : k.rows[kind][p.tile], align_up(row_tiles * g.column_tiles * p.splits, 8), t.threads, stream, g);
-    if (p.splits == 1) return;
-    EpSumSplitsArgs s{};
-    s.layout = l;
-    s.partial = g.partial;
-    s.out = g.out;
-    s.out_ld = g.out_ld;
-    s.splits = p.splits;
-    s.num_columns = g.num_columns;
-    launch(k.sum_splits, ceil_div((int64_t)l.num_rows * ceil_div(g.num_columns, 512), 4), 256, stream, s);
+    const int64_t blocks = align_up(row_tiles * g.column_tiles * p.splits, 8);
+    const int ranks = g.lora.rank <= 16 ? 0 : g.lora.rank <= 32 ? 1 : 2;
+    if (p.splits == 1) {
+        if (lora != nullptr) launch(lora->rows == 16 ? k.lora_down[ranks] : k.lora_down_rows, g.lora.blocks, 256, stream, g);
+        launch(k.rows[kind][p.tile], blocks, t.threads, stream, g);
+        return;
+    }
+    if (lora != nullptr) {
+        EP_HOST_ASSERT(lora->rows == 16);
+        launch(k.split_lora[ranks], g.lora.blocks + blocks, t.threads, stream, g);
+    } else {
+        launch(k.split[kind], blocks, t.threads, stream, g);
+    }
+    launch(lora != nullptr ? k.sum_splits_lora : k.sum_splits, ceil_div((int64_t)l.num_rows * ceil_div(g.num_columns, 512), 4), 256, stream, g);
 }
 
-int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns,
-                                          int dtype) {
+int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns) {
     if (num_rows <= 0 or num_rows > INT32_MAX or num_experts <= 0 or expert_alignment <= 0 or depth <= 0 or depth > INT32_MAX / 2 or num_columns <= 0 or
         num_columns > INT32_MAX / 2)
         return 0;
-    const Plan p = plan_rows(num_rows, num_experts, expert_alignment, depth, num_columns, dtype == EP_DTYPE_FP8_E4M3, false);
+    const Plan p = plan_rows(num_rows, num_experts, expert_alignment, depth, num_columns, false);
     return p.splits > 1 ? (int64_t)p.splits * num_rows * num_columns * 4 : 0;
 }
 
@@ -234,25 +254,9 @@ int ep_grouped_linear(const ep_grouped_linear_args_t* args) {
         EP_HOST_ASSERT(args != nullptr);
         EpGemmArgs g = linear_args(args);
         if (g.layout.num_rows == 0) return;
-        launch_rows(g, args->x.dtype == EP_DTYPE_FP8_E4M3 ? kKindFp8 : args->transpose_weight ? kKindTransposed : kKindBf16, args->workspace,
-                    args->workspace_bytes, args->stream);
+        launch_rows(g, args->x.dtype == EP_DTYPE_FP8_E4M3 ? kKindFp8 : args->transpose_weight ? kKindTransposed : kKindBf16, nullptr,
+                    args->workspace, args->workspace_bytes, args->stream);
     });
-}
-
-// How the rows times the adapters' first matrices are split: rows of a workgroup's tile, chunks of the depth, workgroups that share the
-// adapters of a tile.
-struct LoraPlan {
-    int rows, chunks, chunk_depth, slots;
-};
-static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
-    LoraPlan p{};
-    p.rows = rows <= 2048 ? 16 : 32;
-    const int64_t tiles = std::max<int64_t>(1, rows / p.rows + std::min<int64_t>(num_experts, rows));
-    p.slots = (int)std::clamp<int64_t>(ceil_div(512, tiles), 1, std::min<int64_t>(p.rows, std::max<int64_t>(rows, 1)));
-    const int64_t steps = ceil_div(depth, EP_LORA_STEP), chunks = std::clamp<int64_t>(ceil_div(512, tiles * p.slots), 1, std::min<int64_t>(steps, 16));
-    p.chunk_depth = (int)(ceil_div(steps, chunks) * EP_LORA_STEP);
-    p.chunks = (int)ceil_div(depth, p.chunk_depth);
-    return p;
 }
 
 int64_t ep_grouped_lora_workspace_bytes(int64_t num_rows, int num_experts, int64_t depth, int rank) {
@@ -300,11 +304,13 @@ int ep_grouped_lora_linear(const ep_grouped_lora_args_t* args) {
         l.chunks = plan.chunks;
         l.chunk_depth = plan.chunk_depth;
         l.slots = plan.slots;
-        const ExpertKernels& k = kernels();
-        const int64_t tiles = row_tiles_bound(g.layout.num_rows, g.layout.num_experts, plan.rows);
-        launch(k.lora_down[plan.rows == 16 ? 0 : 1][rank <= 16 ? 0 : rank <= 32 ? 1 : 2], tiles * plan.chunks * plan.slots, 256,
-               args->linear.stream, g);
-        launch_rows(g, kKindLora, args->linear.workspace, args->linear.workspace_bytes, args->linear.stream);
+        const int64_t blocks = row_tiles_bound(g.layout.num_rows, g.layout.num_experts, plan.rows) * plan.chunks * plan.slots;
+        EP_HOST_ASSERT(blocks <= INT32_MAX / 2);
+        l.blocks = (int)blocks;
+        // (one buffer of 31 bits has to reach all of them)
+        const bool near = (int64_t)l.num_adapters * l.down_adapter + 64 * l.down_ld < INT32_MAX;
+        l.together = near ? (int)(64 / rank) : 1;
+        launch_rows(g, kKindLora, &plan, args->linear.workspace, args->linear.workspace_bytes, args->linear.stream);
     });
 }
 
@@ -364,6 +370,7 @@ int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
         g.column_tiles = (int)ceil_div(g.num_columns, tile);
         g.row_tiles = (int)ceil_div(g.num_out_rows, tile);
         g.accumulate = args->accumulate != 0;
+        g.few_rows = mean_rows(g.layout.num_rows, g.layout.num_experts, g.layout.alignment) <= 256;
         const int64_t tiles = (int64_t)g.layout.num_experts * g.row_tiles;
         EP_HOST_ASSERT(tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles));
         launch(kernels().weights[f32 ? 1 : 0][large ? 1 : 0], align_up(tiles * g.column_tiles, 8), 512, args->stream, g);
@@ -407,7 +414,7 @@ int ep_swiglu(const ep_swiglu_args_t* args) {
             s.sf_col = sf.stride[1];
         }
         if (s.layout.num_rows == 0) return;
-        s.parts_per_task = s.num_parts;
+        s.parts_per_task = (int)std::clamp<int64_t>((int64_t)s.layout.num_rows * s.num_parts / 8192, 1, s.num_parts);
         const int64_t tasks = (int64_t)s.layout.num_rows * ceil_div(s.num_parts, s.parts_per_task);
         launch(kernels().swiglu[fp8 ? 1 : 0], ceil_div(tasks, 4), 256, args->stream, s);
     });

@@ -8,6 +8,12 @@
 #include "ep_expert_args.h"
 
 #define WAVE 64
+// Loads and stores of what is touched once: past the caches.
+template <bool NT, typename T>
+__device__ __forceinline__ void store(T* p, T v) {
+    if (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -104,7 +110,8 @@ __device__ __forceinline__ RowTile find_row_tile(const EpExpertLayout& l, int ti
 }
 
 // 0: not a row to write, 1: one to write zeros into, 2: a row of an expert
-__device__ __forceinline__ int kind_of_row(const EpExpertLayout& l, int row) {
+__device__ __forceinline__ int kind_of_row(const EpExpertLayout& l, int row, int& expert) {
+    expert = 0;
     if (l.psum == nullptr) return 2;
     // experts that end at or before the row, and where the last of them ends
     int before = 0, end = 0;
@@ -118,14 +125,15 @@ __device__ __forceinline__ int kind_of_row(const EpExpertLayout& l, int row) {
     }
     const int start = align_up(max(end, 0), l.alignment);
     if (row < start) return l.zero_rows != EP_ZERO_NONE ? 1 : 0;
+    expert = before;
     return before < l.num_experts ? 2 : l.zero_rows == EP_ZERO_ALL ? 1 : 0;
 }
 
 // Workgroup -> tile.  Workgroups go round the eight XCDs, each with an L2 of its own: an XCD takes one stretch of the tiles, and
 // within a stretch GROUP row tiles go through the column tiles together, so that what runs at once on an XCD reads few panels.
-__device__ __forceinline__ bool tile_of_block(int row_tiles, int column_tiles, int group, int& row, int& column) {
+__device__ __forceinline__ bool tile_of_block(int block, int row_tiles, int column_tiles, int group, int& row, int& column) {
     const int total = row_tiles * column_tiles, share = ceil_div(total, 8);
-    const int at = (int)blockIdx.x >> 3, id = ((int)blockIdx.x & 7) * share + at;
+    const int at = block >> 3, id = (block & 7) * share + at;
     if (at >= share || id >= total) return false;
     const int g = id / (group * column_tiles), first = g * group, rows = min(group, row_tiles - first);
     const int in = id - g * group * column_tiles;
@@ -152,6 +160,14 @@ __device__ __forceinline__ i32x4 buffer_of(const char* base, unsigned bytes) {
     return i32x4{(int)(unsigned)at, (int)((unsigned)(at >> 32) & 0xffffu), (int)bytes, 0x00020000};
 }
 
+// (rows and channels that do not exist come as zeros)
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t bounded(const char* base, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(buffer_t buffer, unsigned from) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)from, 0, 0));
+}
 // (No register is written: nothing that the compiler could use before the data are there.  What was fetched is read behind
 // wait_and_meet.)
 __device__ __forceinline__ void fetch16(unsigned to, unsigned from, i32x4 buffer) {
@@ -283,29 +299,36 @@ __device__ __forceinline__ f32x16 multiply_add_fp8(const Chunks& c, const Chunks
 
 // ---- low-rank adapters: numbers of a tile ------------------------------------------------------------------
 
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) v = min(v, __shfl_xor(v, d));
-    return v;
-}
 constexpr int NO_ADAPTER = 0x7fffffff;
-// The smallest number of the tile's rows above `last`; every wave finds it by itself.
-template <int TM>
-__device__ __forceinline__ int next_adapter(const int* of_row, int last) {
+__device__ __forceinline__ int adapter_of(const EpLoraArgs& l, int64_t first, int row, int valid) {
+    const int a = row < valid ? l.adapter[first + row] : -1;
+    return a >= 0 && a < l.num_adapters ? a : NO_ADAPTER;
+}
+__device__ __forceinline__ int wave_min(int v) {
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));      // row_shr:1
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));      // row_shr:2
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));      // row_shr:4
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));      // row_shr:8
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));      // row_bcast:15 to rows 1 and 3
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));      // row_bcast:31 to rows 2 and 3
+    return __builtin_amdgcn_readlane(v, WAVE - 1);
+}
+// The smallest number above `last` of a tile's rows, a wave's lanes holding 64 rows' numbers each time.
+template <int N>
+__device__ __forceinline__ int next_adapter(const int (&of_row)[N], int last) {
     int v = NO_ADAPTER;
 #pragma unroll
-    for (int i = 0; i < TM; i += WAVE) {
-        const int r = i + lane_id();
-        const int a = r < TM ? of_row[r] : NO_ADAPTER;
-        v = min(v, a > last ? a : NO_ADAPTER);
-    }
-    return uniform(wave_min(v));
+    for (int i = 0; i < N; ++i) v = min(v, of_row[i] > last ? of_row[i] : NO_ADAPTER);
+    return wave_min(v);
 }
-template <int TM>
-__device__ __forceinline__ void note_adapters(const EpLoraArgs& l, int first, int valid, int* of_row, int threads) {
-    for (int r = threadIdx.x; r < TM; r += threads) {
-        const int a = r < valid ? l.adapter[first + r] : -1;
-        of_row[r] = a >= 0 && a < l.num_adapters ? a : NO_ADAPTER;
+
+// Eight ranks of a low-rank row.
+__device__ __forceinline__ void low_ranks(const EpGemmArgs& a, int64_t row, int rank, f32x4 (&sum)[2]) {
+    sum[0] = sum[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < a.lora.chunks; ++k) {
+        const f32x4* const from = (const f32x4*)(a.lora.low + ((k * (int64_t)a.layout.num_rows + row) * a.lora.rank + rank));
+        sum[0] += from[0];
+        sum[1] += from[1];
     }
 }
 
@@ -313,7 +336,8 @@ __device__ __forceinline__ void note_adapters(const EpLoraArgs& l, int first, in
 //
 // One workgroup computes TM x TN of the output, WR x WC waves a part each, in 32 bits.  The matrix instruction's first operand is
 // the output's columns, its second the rows: a lane then holds four neighbouring columns of one row.
-template <int TM, int TN, int WR, int WC, int MT, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false>
+template <int TM, int TN, int WR, int WC, int MT, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false,
+          bool LOW_RANK = false>
 struct Gemm {
     static constexpr int WAVES = WR * WC, FM = TM / WR, FN = TN / WC, NR = FM / MT, NC = FN / MT;
     static constexpr int Q = MT / 8, HQ = Q / 2;      // fragments of a step and of half of one
@@ -328,16 +352,18 @@ struct Gemm {
     typedef TileFetch<TM, WAVES, ROWS_T> RowsFetch;
     static constexpr int FETCHES = ColumnsFetch::MINE + RowsFetch::MINE + (FP8 ? 1 : 0);       // of a wave and step
     static constexpr int STEP = FP8 ? 128 : 64;
+    // Results past the caches: those of large tiles are more than the L2 holds next to the operands (gradients of 64 experts' weights of
+    // 1536 x 2560 from 7147 rows 250 -> 186 us, the FP8 product of 98304 rows 3402 -> 3340; the others are level).
+    static constexpr bool STREAM = ROWS_T || TM >= 256;
     // fetches that a wave may have left when the rows and columns of a step have to be there, `ahead` steps before the newest
     static constexpr int pending(int ahead) { return ahead * FETCHES + (SC > SR ? ColumnsFetch::MINE : 0); }
 
     // rows .. rows + valid: what is computed, up to limit zeros are written; columns from column on
     __device__ __forceinline__ static void run(const EpGemmArgs& a, const char* rows, const char* columns, int valid, int limit,
                                                int num_columns, int depth, const float* rows_sf, const float* columns_sf, char* out,
-                                               int64_t out_ld, int first = 0, const char* up = nullptr) {
+                                               int64_t out_ld, int64_t first = 0, const char* up = nullptr, int numbers = NO_ADAPTER) {
         __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];
         __shared__ float table[FP8 ? BLOCKS * TABLE : 1];
-        __shared__ int adapters[LORA ? TM : 1];
         const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
         const int first_row = (wave / WC) * FM, first_column = (wave % WC) * FN;
         const unsigned lds0 = (unsigned)(size_t)(lds_byte*)lds;
@@ -354,6 +380,25 @@ struct Gemm {
         RowsFetch rf;
         cf.init(columns, a.columns_ld, min(num_columns, TN), depth, FP8 ? 1 : 2, wave);
         rf.init(rows, a.rows_ld, valid, depth, FP8 ? 1 : 2, wave);
+        if constexpr (LOW_RANK) {
+            // columns: the adapters' matrices one below the other, lane j of `numbers` has the number of the j-th
+            const EpLoraArgs& l = a.lora;
+            const int base = __builtin_amdgcn_readlane(numbers, 0);
+            int last = base;
+#pragma unroll
+            for (int i = 0; i < TN / 8; ++i) {
+                const int n = __builtin_amdgcn_readlane(numbers, i);
+                last = n != NO_ADAPTER ? n : last;
+            }
+            cf.bytes = (unsigned)((last - base) * l.down_adapter + (l.rank - 1) * l.down_ld) + depth * 2;
+#pragma unroll
+            for (int i = 0; i < ColumnsFetch::MINE; ++i) {
+                const int r = ColumnsFetch::piece(i, wave) * 8, j = r / l.rank;      // (eight ranks of one adapter)
+                const int n = __builtin_amdgcn_readlane(numbers, j);
+                cf.from[i] = n == NO_ADAPTER ? OUTSIDE
+                                             : (unsigned)((n - base) * l.down_adapter + (r - j * l.rank + (lane >> 3)) * l.down_ld) + cf.chunk * 16;
+            }
+        }
         unsigned sf_from = 0, sf_bytes = 0;
         const int groups = ceil_div(depth, 128);
         constexpr int SF_PIECES = SF_BYTES / 256 > 0 ? SF_BYTES / 256 : 1;
@@ -414,17 +459,27 @@ struct Gemm {
 #pragma unroll
             for (int s = 0; s < SR - 1; ++s) fetch_all(begin_fetch(s, s, s + SC - SR, s + SC - SR), 0);
         }
-        if (LORA && up != nullptr) {
-            add_adapters(a, lds + (SC - 1) * COLUMNS_BYTES, lds + ROWS_AT + (SR - 1) * ROWS_BYTES, adapters, first, valid, num_columns, up, [&] {
-                u32x4 c[HQ][NC], r[HQ][NR];
+        // The adapters' part: here for few adapters, behind the product for many.
+        bool by_row = false;
+        if (LORA) {
+            int of_row[(TM + WAVE - 1) / WAVE];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+            for (int i = 0; i < (TM + WAVE - 1) / WAVE; ++i) of_row[i] = i * WAVE + lane < TM ? adapter_of(a.lora, first, i * WAVE + lane, valid) : NO_ADAPTER;
+            int number = next_adapter(of_row, -1);
+            for (int i = 0; i < FEW_ADAPTERS && number != NO_ADAPTER; ++i) number = next_adapter(of_row, number);
+            by_row = number != NO_ADAPTER;
+            if (!by_row) {
+                add_adapters(a, lds + (SC - 1) * COLUMNS_BYTES, lds + ROWS_AT + (SR - 1) * ROWS_BYTES, of_row, first, valid, num_columns, up, [&] {
+                    u32x4 c[HQ][NC], r[HQ][NR];
 #pragma unroll
-                    for (int i = 0; i < READS; ++i) read_one(c, r, SR - 1, SC - 1, half, i);
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int i = 0; i < PRODUCTS; ++i) multiply_one(c, r, i);
-                }
-            });
+                        for (int i = 0; i < READS; ++i) read_one(c, r, SR - 1, SC - 1, half, i);
+#pragma unroll
+                        for (int i = 0; i < PRODUCTS; ++i) multiply_one(c, r, i);
+                    }
+                });
+            }
         }
         if (steps > 0 && !(FP8 && NR >= 4)) fetch_all(begin_fetch(SR - 1, SR - 1, SC - 1, SC - 1), 0);
         if constexpr (!FP8) {
@@ -588,11 +643,17 @@ struct Gemm {
             }
         }
         wait_and_meet<0>();      // (the last fetches, of zeros, land in LDS too)
+        if (LORA && by_row) add_adapters_by_row(a, acc, up, first, valid, first_row, first_column, num_columns);
 
         // MT rows of a wave's part at a time through LDS, to leave as whole lines
         char* const mine = lds + wave * MT * OUT_ROW;
         constexpr int LANES = FN * OUT_ELEM / 16, PASS = WAVE / LANES;      // lanes of a row, rows of a store
         const int piece = lane % LANES, column = first_column + piece * (16 / OUT_ELEM);
+        int segment = 0, of_segment = NO_ADAPTER;      // of the adapters' ranks: which adapter's this lane stores
+        if constexpr (LOW_RANK) {
+            segment = column / a.lora.rank;
+            of_segment = __shfl(numbers, segment);
+        }
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
 #pragma unroll
@@ -614,38 +675,50 @@ struct Gemm {
                 u32x4 v = *(const u32x4*)(mine + in * OUT_ROW + piece * 16);
                 if (r >= valid) v = u32x4{0u, 0u, 0u, 0u};
                 u32x4* const to = (u32x4*)(out + (r * out_ld + column) * OUT_ELEM);
+                if constexpr (LOW_RANK) {
+                    // only the rows that have the adapter
+                    const int mine = adapter_of(a.lora, first, r, valid);
+                    if (mine == NO_ADAPTER || mine != of_segment) continue;
+                    const float scale = a.lora.scales != nullptr ? a.lora.scales[mine] : 1.0f;
+                    *(f32x4*)((float*)out + (int64_t)r * a.lora.rank + (column - segment * a.lora.rank)) = __builtin_bit_cast(f32x4, v) * scale;
+                    continue;
+                }
                 if (OUT32 && a.accumulate) {
                     const f32x4 sum = *(const f32x4*)to + __builtin_bit_cast(f32x4, v);
                     v = __builtin_bit_cast(u32x4, sum);
                 }
-                *to = v;
+                store<STREAM>(to, v);
             }
             asm volatile("" ::: "memory");
         }
     }
 
-    // The adapters' part, in front of the product's first step and in the LDS of its last stage, while the first ones are on their way: for
+    // Few adapters: in front of the product's first step and in the LDS of its last stage, while the first ones are on their way.  For
     // every adapter that rows of the tile have, 32 ranks at a time, a step of 64 channels.  The low-rank rows are sums in 32 bits; they
-    // go in as two BF16, the rounded value and the rest, against the same column of `up` twice, which keeps 2^-17 of them.
+    // go in as two BF16, the rounded value and the rest, against the same column of `up` twice, which keeps 2^-17 of them.  A step
+    // takes about 2.5 us, most of it the way of its operands.
+    static constexpr int FEW_ADAPTERS = TM >= 256 ? 8 : 4;
     template <typename Multiply>
-    __device__ __forceinline__ static void add_adapters(const EpGemmArgs& a, char* to_columns, char* to_rows, int* of_row, int first, int valid, int num_columns,
-                                                        const char* up, Multiply multiply) {
-        constexpr int THREADS = WAVES * WAVE;
+    __device__ __forceinline__ static void add_adapters(const EpGemmArgs& a, char* to_columns, char* to_rows, const int (&of_row)[(TM + WAVE - 1) / WAVE],
+                                                        int64_t first, int valid, int num_columns, const char* up, Multiply multiply) {
+        constexpr int THREADS = WAVES * WAVE, MINE = (TM * 4 + THREADS - 1) / THREADS;
         const EpLoraArgs& l = a.lora;
-        note_adapters<TM>(l, first, valid, of_row, THREADS);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        for (int number = next_adapter<TM>(of_row, -1); number != NO_ADAPTER; number = next_adapter<TM>(of_row, number)) {
+        int mine[MINE];           // adapters of the rows that this thread brings
+#pragma unroll
+        for (int n = 0; n < MINE; ++n) {
+            const int r = (threadIdx.x + n * THREADS) >> 2;
+            mine[n] = r < TM ? adapter_of(l, first, r, valid) : NO_ADAPTER;
+        }
+        for (int number = next_adapter(of_row, -1); number != NO_ADAPTER; number = next_adapter(of_row, number)) {
             for (int r0 = 0; r0 < l.rank; r0 += 32) {
-                for (int i = threadIdx.x; i < TM * 4; i += THREADS) {
-                    const int r = i >> 2, c = i & 3, rank = r0 + c * 8;
+#pragma unroll
+                for (int n = 0; n < MINE; ++n) {
+                    const int i = threadIdx.x + n * THREADS, r = i >> 2, c = i & 3, rank = r0 + c * 8;
+                    if (r >= TM) continue;
                     bf16x8 high = {}, rest = {};
-                    if (of_row[r] == number && rank < l.rank) {
-                        f32x4 sum[2] = {};
-                        for (int k = 0; k < l.chunks; ++k) {
-                            const f32x4* const from = (const f32x4*)(l.low + (((int64_t)k * a.layout.num_rows + first + r) * l.rank + rank));
-                            sum[0] += from[0];
-                            sum[1] += from[1];
-                        }
+                    if (mine[n] == number && rank < l.rank) {
+                        f32x4 sum[2];
+                        low_ranks(a, first + r, rank, sum);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const float v = sum[j >> 2][j & 3];
@@ -671,14 +744,44 @@ struct Gemm {
             }
         }
     }
+    // Many adapters: behind the product, lane by lane with the row's own adapter, eight ranks at a time and four columns of a sum together.  The
+    // time goes by the ranks and not by the number of adapters (64 rows of 27 adapters beside 128 columns: a step each was 70 us).
+    __device__ __forceinline__ static void add_adapters_by_row(const EpGemmArgs& a, typename Sums<MT>::type (&acc)[NR][NC], const char* up, int64_t first,
+                                                               int valid, int first_row, int first_column, int num_columns) {
+        const EpLoraArgs& l = a.lora;
+        const int lane = lane_id();
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int row = first_row + i * MT + lane % MT, number = adapter_of(l, first, row, valid);
+            if (number == NO_ADAPTER) continue;
+            const char* const mine = up + number * l.up_adapter;
+            for (int rank = 0; rank < l.rank; rank += 8) {
+                f32x4 low[2];
+                low_ranks(a, first + row, rank, low);
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+#pragma unroll
+                    for (int g = 0; g < MT * MT / WAVE; ++g) {
+                        const int column = first_column + j * MT + g / 4 * (WAVE / MT * 4) + lane / MT * 4 + g % 4;
+                        if (column >= num_columns) continue;
+                        const bf16x8 w = *(const bf16x8*)(mine + column * l.up_ld + rank * 2);
+                        float sum = acc[i][j][g];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(low[k >> 2][k & 3], (float)w[k], sum);
+                        acc[i][j][g] = sum;
+                    }
+                }
+            }
+        }
+    }
 
     // Rows of the layout times the weights of their expert: out[r, c] = sum_d rows[r, d] columns[e(r)][c, d].  SPLIT: of a part of
     // the depth, in 32 bits; ep_sum_splits adds the parts.
     template <bool SPLIT>
-    __device__ __forceinline__ static void rows_kernel(const EpGemmArgs& a, int group) {
+    __device__ __forceinline__ static void rows_kernel(const EpGemmArgs& a, int group, int block = blockIdx.x) {
         const int row_tiles = count_row_tiles<TM>(a.layout);
         int row, column, part = 0;
-        if (!tile_of_block(row_tiles, SPLIT ? a.column_tiles * a.splits : a.column_tiles, group, row, column)) return;
+        if (!tile_of_block(block, row_tiles, SPLIT ? a.column_tiles * a.splits : a.column_tiles, group, row, column)) return;
         const RowTile t = find_row_tile<TM>(a.layout, row);
         int64_t d0 = 0;
         int depth = a.depth, limit = t.limit;
@@ -698,13 +801,21 @@ struct Gemm {
             a.rows_sf + (FP8 ? t.first * a.rows_sf_row + d0 / 128 * a.rows_sf_col : 0),
             a.columns_sf + (FP8 ? t.expert * a.columns_sf_expert + c0 / 128 * a.columns_sf_row + d0 / 128 * a.columns_sf_col : 0),
             out + (t.first * out_ld + c0) * OUT_ELEM, out_ld, t.first,
-            LORA && part == 0 ? a.lora.up + t.expert * a.lora.up_expert + c0 * a.lora.up_ld : nullptr);
+            LORA ? a.lora.up + t.expert * a.lora.up_expert + c0 * a.lora.up_ld : nullptr);
     }
 
     // Gradient of an expert's weights: out[e][r, c] = sum over the expert's rows d of rows[d, r] columns[d, c]
     __device__ __forceinline__ static void weights_kernel(const EpGemmArgs& a, int group) {
         int row, column;
-        if (!tile_of_block(a.row_tiles * a.layout.num_experts, a.column_tiles, group, row, column)) return;
+        const int row_tiles = a.row_tiles * a.layout.num_experts;
+        if (a.few_rows) {
+            // the time is the results': the tiles of an expert with many rows go to all XCDs
+            if ((int)blockIdx.x >= row_tiles * a.column_tiles) return;
+            row = blockIdx.x / a.column_tiles;
+            column = blockIdx.x - row * a.column_tiles;
+        } else if (!tile_of_block(blockIdx.x, row_tiles, a.column_tiles, group, row, column)) {
+            return;
+        }
         const int e = row / a.row_tiles, r0 = (row - e * a.row_tiles) * TM, c0 = column * TN;
         const ExpertRows in = rows_of_expert(a.layout, e);
         const int count = uniform(in.count);
@@ -719,10 +830,10 @@ struct Gemm {
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
         Gemm<TM, TN, WR, WC, MT, SR, SC, FP8, COLUMNS_T, false, false>::rows_kernel<false>(a, GROUP);                 \
     }
-#define EP_GEMM_SPLIT(NAME, TM, TN, WR, WC, MT, SR, SC, FP8, LORA, GROUP)                                             \
-    extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, MT, SR, SC, FP8, false, false, true, LORA>::rows_kernel<true>(a, GROUP);                 \
-    }
+typedef Gemm<64, 128, 2, 2, 16, 3, 3, false, false, false, true> SplitBf16;
+typedef Gemm<64, 128, 2, 2, 16, 3, 3, true, false, false, true> SplitFp8;
+extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_bf16(EpGemmArgs a) { SplitBf16::rows_kernel<true>(a, 1); }
+extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_fp8(EpGemmArgs a) { SplitFp8::rows_kernel<true>(a, 1); }
 #define EP_GEMM_LORA(NAME, TM, TN, WR, WC, MT, SR, SC, GROUP)                                                         \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
         Gemm<TM, TN, WR, WC, MT, SR, SC, false, false, false, false, true>::rows_kernel<false>(a, GROUP);             \
@@ -733,82 +844,89 @@ struct Gemm {
     }
 EP_GEMM_ROWS(ep_grouped_bf16_32x64, 32, 64, 1, 4, 16, 4, 4, false, false, 4)
 EP_GEMM_ROWS(ep_grouped_bf16_64x128, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
-EP_GEMM_ROWS(ep_grouped_bf16_128x128, 128, 128, 2, 4, 16, 3, 3, false, false, 4)
+EP_GEMM_ROWS(ep_grouped_bf16_64x256, 64, 256, 1, 8, 16, 3, 3, false, false, 1)
+EP_GEMM_ROWS(ep_grouped_bf16_128x256, 128, 256, 2, 4, 16, 3, 3, false, false, 1)
 EP_GEMM_ROWS(ep_grouped_bf16_256x256, 256, 256, 4, 2, 16, 2, 3, false, false, 8)
 EP_GEMM_ROWS(ep_grouped_fp8_32x64, 32, 64, 1, 4, 16, 4, 4, true, false, 4)
 EP_GEMM_ROWS(ep_grouped_fp8_64x128, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
-EP_GEMM_ROWS(ep_grouped_fp8_128x128, 128, 128, 2, 4, 16, 3, 3, true, false, 4)
+EP_GEMM_ROWS(ep_grouped_fp8_64x256, 64, 256, 1, 8, 16, 3, 3, true, false, 1)
+EP_GEMM_ROWS(ep_grouped_fp8_128x256, 128, 256, 2, 4, 16, 3, 3, true, false, 1)
 EP_GEMM_ROWS(ep_grouped_fp8_256x256, 256, 256, 2, 4, 16, 2, 2, true, false, 8)
-EP_GEMM_ROWS(ep_grouped_transposed_128x128, 128, 128, 2, 4, 16, 3, 3, false, true, 4)
+EP_GEMM_ROWS(ep_grouped_transposed_128x256, 128, 256, 2, 4, 16, 3, 3, false, true, 1)
 EP_GEMM_ROWS(ep_grouped_transposed_256x256, 256, 256, 2, 4, 16, 2, 3, false, true, 8)
-EP_GEMM_SPLIT(ep_grouped_split_bf16, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
-EP_GEMM_SPLIT(ep_grouped_split_fp8, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
-EP_GEMM_SPLIT(ep_grouped_split_lora, 64, 128, 2, 2, 16, 3, 3, false, true, 1)
 EP_GEMM_LORA(ep_grouped_lora_32x64, 32, 64, 1, 4, 16, 4, 4, 4)
 EP_GEMM_LORA(ep_grouped_lora_64x128, 64, 128, 2, 2, 16, 3, 3, 1)
-EP_GEMM_LORA(ep_grouped_lora_128x128, 128, 128, 2, 4, 16, 3, 3, 4)
-EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 16, 2, 2, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 3, 3, false, 8)
+EP_GEMM_LORA(ep_grouped_lora_64x256, 64, 256, 1, 8, 16, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_128x256, 128, 256, 2, 4, 16, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 16, 2, 3, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 2, 2, false, 8)
 EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 16, 2, 3, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 3, 3, true, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 2, 2, true, 8)
 EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 16, 2, 3, true, 8)
 
 // ---- low-rank adapters: rows times the first matrix ---------------------------------------------------------
 //
 // low[chunk][r] = scale[a] * sum over the chunk's channels of down[a][e] rows[r].  A workgroup has ROWS rows of an expert, a chunk of the
-// depth, which its four waves share 128 channels at a time, and every `slots`-th of the adapters that its rows have: all rows are
+// depth, which its four waves share 64 or 128 channels at a time, and every `slots`-th of the adapters that its rows have: all rows are
 // multiplied with an adapter's matrix, and the rows that have it keep what they get.  Operands go from memory straight to
 // registers: nothing is used twice but by the neighbouring waves, out of the caches.
 template <int ROWS, int RANKS>
-__device__ __forceinline__ void lora_down_body(const EpGemmArgs& a) {
-    constexpr int NR = ROWS / 16, NK = RANKS / 16, PARTS = EP_LORA_STEP / 128;
-    __shared__ int of_row[ROWS];
+__device__ __forceinline__ void lora_down_body(const EpGemmArgs& a, int block) {
+    constexpr int NR = ROWS / 16, NK = RANKS / 16, PARTS = RANKS > 32 ? 2 : 4;
     __shared__ __attribute__((aligned(16))) float sums[4][ROWS][RANKS + 4];
     const EpLoraArgs& l = a.lora;
     const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
-    int at = blockIdx.x;
+    int at = block;
     const int slot = at % l.slots;
     at /= l.slots;
     const int chunk = at % l.chunks, tile = at / l.chunks;
     const RowTile t = find_row_tile<ROWS>(a.layout, tile);
     if (t.valid <= 0) return;
-    note_adapters<ROWS>(l, t.first, t.valid, of_row, 256);
-    __syncthreads();
+    // every wave: the rows' adapters, and of each the first row that has it
+    const int of_row = lane < ROWS ? adapter_of(l, t.first, lane, t.valid) : NO_ADAPTER;
+    bool leads = of_row != NO_ADAPTER;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) leads = leads && !(lane > i && __builtin_amdgcn_readlane(of_row, i) == of_row);
     const int begin = chunk * l.chunk_depth, end = min(begin + l.chunk_depth, a.depth);
-    const char* const rows = a.rows + t.first * a.rows_ld;
+    const buffer_t x_buffer = bounded(a.rows + t.first * a.rows_ld, (unsigned)((t.valid - 1) * a.rows_ld) + a.depth * 2);
     int n = 0;
-    for (int number = next_adapter<ROWS>(of_row, -1); number != NO_ADAPTER; number = next_adapter<ROWS>(of_row, number)) {
+    for (uint64_t leaders = __ballot(leads); leaders != 0; leaders &= leaders - 1) {
         if (n++ % l.slots != slot) continue;
-        const char* const down = l.down + number * l.down_adapter + t.expert * l.down_expert;
+        const int number = __builtin_amdgcn_readlane(of_row, __builtin_ctzll(leaders));
+        const buffer_t w_buffer = bounded(l.down + number * l.down_adapter + t.expert * l.down_expert, (unsigned)((l.rank - 1) * l.down_ld) + a.depth * 2);
         f32x4 acc[NR][NK];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int k0 = begin + wave * 32 * PARTS; k0 < end; k0 += 128 * PARTS) {
-            u32x4 x[PARTS][NR], w[PARTS][NK];
+        // (a turn's operands are on their way while the one before is multiplied)
+        u32x4 x[2][PARTS][NR], w[2][PARTS][NK];
+        auto load = [&](int k0, u32x4 (&x)[PARTS][NR], u32x4 (&w)[PARTS][NK]) {
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 const int k = k0 + p * 32 + (lane >> 4) * 8;
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    const int r = i * 16 + (lane & 15);
-                    x[p][i] = r < t.valid && k < end ? *(const u32x4*)(rows + r * a.rows_ld + (int64_t)k * 2) : u32x4{0u, 0u, 0u, 0u};
-                }
+                for (int i = 0; i < NR; ++i) x[p][i] = load16(x_buffer, k < end ? (unsigned)((i * 16 + (lane & 15)) * a.rows_ld) + k * 2 : OUTSIDE);
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    const int r = j * 16 + (lane & 15);
-                    w[p][j] = r < l.rank && k < end ? *(const u32x4*)(down + r * l.down_ld + (int64_t)k * 2) : u32x4{0u, 0u, 0u, 0u};
-                }
+                for (int j = 0; j < NK; ++j) w[p][j] = load16(w_buffer, k < end ? (unsigned)((j * 16 + (lane & 15)) * l.down_ld) + k * 2 : OUTSIDE);
             }
+        };
+        auto multiply = [&](const u32x4 (&x)[PARTS][NR], const u32x4 (&w)[PARTS][NK]) {
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
 #pragma unroll
-                    for (int j = 0; j < NK; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[p][j]),
-                                                                            __builtin_bit_cast(bf16x8, x[p][i]), acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NK; ++j) acc[i][j] = multiply_add(w[p][j], x[p][i], acc[i][j]);
+        };
+        constexpr int TURN = 128 * PARTS;
+        const int k0 = begin + wave * 32 * PARTS;
+        load(k0, x[0], w[0]);
+        for (int k = k0; k < end; k += 2 * TURN) {
+            load(k + TURN, x[1], w[1]);
+            multiply(x[0], w[0]);
+            load(k + 2 * TURN, x[0], w[0]);
+            multiply(x[1], w[1]);
         }
 #pragma unroll
         for (int i = 0; i < NR; ++i)
@@ -818,7 +936,7 @@ __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a) {
         const float scale = l.scales != nullptr ? l.scales[number] : 1.0f;
         for (int i = threadIdx.x; i < ROWS * (RANKS / 4); i += 256) {
             const int r = i / (RANKS / 4), c = (i - r * (RANKS / 4)) * 4;
-            if (of_row[r] != number || c >= l.rank) continue;
+            if (__shfl(of_row, r) != number || c >= l.rank) continue;
             const f32x4 sum = (*(const f32x4*)&sums[0][r][c] + *(const f32x4*)&sums[1][r][c]) + (*(const f32x4*)&sums[2][r][c] + *(const f32x4*)&sums[3][r][c]);
             *(f32x4*)(l.low + (((int64_t)chunk * a.layout.num_rows + t.first + r) * l.rank + c)) = sum * scale;
         }
@@ -826,13 +944,48 @@ __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a) {
     }
 }
 #define EP_LORA_DOWN(ROWS, RANKS) \
-    extern "C" __global__ __launch_bounds__(256) void ep_lora_down_##ROWS##_##RANKS(EpGemmArgs a) { lora_down_body<ROWS, RANKS>(a); }
+    extern "C" __global__ __launch_bounds__(256) void ep_lora_down_##ROWS##_##RANKS(EpGemmArgs a) { lora_down_body<ROWS, RANKS>(a, blockIdx.x); }
 EP_LORA_DOWN(16, 16)
 EP_LORA_DOWN(16, 32)
 EP_LORA_DOWN(16, 64)
-EP_LORA_DOWN(32, 16)
-EP_LORA_DOWN(32, 32)
-EP_LORA_DOWN(32, 64)
+
+// Many rows: the same sums as a product of 64 rows with the matrices of as many adapters as have 64 ranks together.
+typedef Gemm<64, 64, 4, 1, 16, 3, 3, false, false, false, true, false, true> LowRank;
+extern "C" __global__ __launch_bounds__(256) void ep_lora_down_rows(EpGemmArgs a) {
+    const EpLoraArgs& l = a.lora;
+    const int chunk = blockIdx.x % l.chunks;
+    const RowTile t = find_row_tile<64>(a.layout, blockIdx.x / l.chunks);
+    if (t.valid <= 0) return;
+    const int of_row[1] = {adapter_of(l, t.first, lane_id(), t.valid)};
+    const int64_t begin = (int64_t)chunk * l.chunk_depth;
+    const int depth = min(l.chunk_depth, a.depth - (int)begin);
+    EpGemmArgs low = a;
+    low.columns_ld = l.down_ld;
+    int number = next_adapter(of_row, -1);
+    while (number != NO_ADAPTER) {
+        const int first = number;
+        int numbers = NO_ADAPTER, count = 0;
+        for (; count < l.together && number != NO_ADAPTER; ++count) {
+            if (lane_id() == count) numbers = number;
+            number = next_adapter(of_row, number);
+        }
+        LowRank::run(low, a.rows + t.first * a.rows_ld + begin * 2, l.down + first * l.down_adapter + t.expert * l.down_expert + begin * 2, t.valid, t.valid,
+                     count * l.rank, depth, nullptr, nullptr, (char*)(l.low + ((int64_t)chunk * a.layout.num_rows + t.first) * l.rank), 0, t.first, nullptr,
+                     numbers);
+        __syncthreads();          // (the next ones' fetches go where rows may still be on their way out)
+    }
+}
+
+// Few tiles: the product in parts of the depth does not need the low-rank rows, ep_sum_splits joins both.  One launch for the two.
+#define EP_LORA_SPLIT(RANKS)                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_lora_##RANKS(EpGemmArgs a) {                   \
+        const int behind = (int)blockIdx.x - ((int)gridDim.x - a.lora.blocks);                                        \
+        if (behind < 0) SplitBf16::rows_kernel<true>(a, 1, blockIdx.x);                                               \
+        else lora_down_body<16, RANKS>(a, behind);                                                                    \
+    }
+EP_LORA_SPLIT(16)
+EP_LORA_SPLIT(32)
+EP_LORA_SPLIT(64)
 
 // ---- a token's number at the rows that it was sent to --------------------------------------------------------
 
@@ -851,27 +1004,54 @@ extern "C" __global__ __launch_bounds__(256) void ep_expand_token_index_rows(EpE
 
 // ---- parts of a depth, added -----------------------------------------------------------------------------
 
-// A lane has eight columns of a row.
-extern "C" __global__ __launch_bounds__(256) void ep_sum_splits(EpSumSplitsArgs a) {
+// A lane has eight columns of a row, and adds what the row's adapter makes of its low-rank row.
+template <bool LORA>
+__device__ __forceinline__ void sum_splits_body(const EpGemmArgs& a) {
     const int vectors = a.num_columns >> 3, per_row = ceil_div(vectors, WAVE);
     const int64_t task = (int64_t)blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
     const int row = uniform((int)(task / per_row)), v = (int)(task - (int64_t)row * per_row) * WAVE + lane_id();
     if (row >= a.layout.num_rows) return;
-    const int kind = kind_of_row(a.layout, row);
-    if (kind == 0 || v >= vectors) return;
+    int expert = 0;
+    const int kind = kind_of_row(a.layout, row, expert);
+    if (kind == 0) return;
     f32x4 sum[2] = {};
     if (kind == 2) {
+        const int number = LORA ? uniform(adapter_of(a.lora, row, 0, 1)) : NO_ADAPTER;
+        // (a lane has a rank of the low-rank row)
+        float low = 0.f;
+        if (LORA && number != NO_ADAPTER && lane_id() < a.lora.rank) {
+#pragma unroll 4
+            for (int k = 0; k < a.lora.chunks; ++k) low += a.lora.low[(k * (int64_t)a.layout.num_rows + row) * a.lora.rank + lane_id()];
+        }
+#pragma unroll 4
         for (int s = 0; s < a.splits; ++s) {
-            const f32x4* const from = (const f32x4*)(a.partial + ((int64_t)s * a.layout.num_rows + row) * a.num_columns) + 2 * v;
+            const f32x4* const from = (const f32x4*)(a.partial + ((int64_t)s * a.layout.num_rows + row) * a.num_columns) + 2 * (v < vectors ? v : 0);
             sum[0] += from[0];
             sum[1] += from[1];
         }
+        if (LORA && number != NO_ADAPTER) {
+            const char* const up = a.lora.up + number * a.lora.up_adapter + expert * a.lora.up_expert + (v < vectors ? v : 0) * 8 * a.lora.up_ld;
+            for (int rank = 0; rank < a.lora.rank; rank += 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bf16x8 w = *(const bf16x8*)(up + i * a.lora.up_ld + rank * 2);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float of_rank = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(low), rank + k));
+                        sum[i >> 2][i & 3] = __builtin_fmaf(of_rank, (float)w[k], sum[i >> 2][i & 3]);
+                    }
+                }
+            }
+        }
     }
+    if (v >= vectors) return;
     bf16x8 out;
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = (__bf16)sum[i >> 2][i & 3];
     *((bf16x8*)(a.out + row * a.out_ld * 2) + v) = out;
 }
+extern "C" __global__ __launch_bounds__(256) void ep_sum_splits(EpGemmArgs a) { sum_splits_body<false>(a); }
+extern "C" __global__ __launch_bounds__(256) void ep_sum_splits_lora(EpGemmArgs a) { sum_splits_body<true>(a); }
 
 // ---- the gated activation -----------------------------------------------------------------------------
 //
@@ -908,44 +1088,56 @@ __device__ __forceinline__ void swiglu_body(const EpSwigluArgs& a) {
     const int per_row = ceil_div(a.num_parts, a.parts_per_task);
     const int row = uniform((int)(task / per_row)), first = uniform((int)(task - (int64_t)row * per_row)) * a.parts_per_task;
     if (row >= a.layout.num_rows) return;
-    const int kind = kind_of_row(a.layout, row);
-    if (kind == 0) return;
-    const float weight = kind == 2 && a.weights != nullptr ? a.weights[row] : 1.0f;
     const u32x4* const h = (const u32x4*)(a.h + (int64_t)row * a.h_ld * 2);
-    const int vectors = a.channels >> 3;
-    for (int part = first; part < min(first + a.parts_per_task, a.num_parts); ++part) {
+    // (the ups begin at a multiple of eight channels as the gates do)
+    const int vectors = a.channels >> 3, end = min(first + a.parts_per_task, a.num_parts);
+    // the first part is on its way while the row is looked up
+    u32x4 next[2];
+    auto fetch = [&](int part) {
+        const int v = part * WAVE + lane;
+        if (v >= vectors) return;
+        next[0] = __builtin_nontemporal_load(h + v);
+        next[1] = __builtin_nontemporal_load(h + vectors + v);
+    };
+    fetch(first);
+    const float of_row = a.weights != nullptr ? a.weights[row] : 1.0f;
+    int expert;
+    const int kind = kind_of_row(a.layout, row, expert);
+    if (kind == 0) return;
+    for (int part = first; part < end; ++part) {
         const int v = part * WAVE + lane;
         const bool live = v < vectors;
         float out[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const u32x4 now[2] = {next[0], next[1]};
+        if (part + 1 < end) fetch(part + 1);
         if (live && kind == 2) {
             float gate[8], up[8];
-            widen(h[v], gate);
-            // (the ups begin at a multiple of eight channels as the gates do)
-            widen(h[vectors + v], up);
+            widen(now[0], gate);
+            widen(now[1], up);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) out[i] = gate[i] * sigmoid(gate[i]) * up[i] * weight;
+            for (int i = 0; i < 8; ++i) out[i] = gate[i] * sigmoid(gate[i]) * up[i] * of_row;
         }
         if constexpr (!FP8) {
-            if (live) ((u32x4*)(a.out + (int64_t)row * a.out_ld * 2))[v] = round_bf16(out);
-            continue;
-        }
-        // the quantiser of the dispatch, of the unrounded values
-        unsigned bits = 0u;
+            if (live) store<true>((u32x4*)(a.out + (int64_t)row * a.out_ld * 2) + v, round_bf16(out));
+        } else {
+            // the quantiser of the dispatch, of the unrounded values
+            unsigned bits = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(out[i]) & 0x7fffffffu);
-        const float m = __uint_as_float(row16_umax(bits));
-        const float amax = m < 1e-4f ? 1e-4f : m;
-        const float inverse = (1.0f / amax) * 448.0f;
-        unsigned q[2];
+            for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(out[i]) & 0x7fffffffu);
+            const float m = __uint_as_float(row16_umax(bits));
+            const float amax = m < 1e-4f ? 1e-4f : m;
+            const float inverse = (1.0f / amax) * 448.0f;
+            unsigned q[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * i] * inverse, out[4 * i + 1] * inverse, 0, false);
-            q[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(out[4 * i + 2] * inverse, out[4 * i + 3] * inverse, w, true);
+            for (int i = 0; i < 2; ++i) {
+                const int w = __builtin_amdgcn_cvt_pk_fp8_f32(out[4 * i] * inverse, out[4 * i + 1] * inverse, 0, false);
+                q[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(out[4 * i + 2] * inverse, out[4 * i + 3] * inverse, w, true);
+            }
+            if (amax != amax) q[0] = q[1] = 0x7f7f7f7fu;
+            if (!live) continue;
+            store<true>((u32x2*)(a.out + (int64_t)row * a.out_ld) + v, u32x2{q[0], q[1]});
+            if ((lane & 15) == 0) a.sf[(int64_t)row * a.sf_row + (int64_t)(v >> 4) * a.sf_col] = kind == 2 ? amax / 448.0f : 0.0f;
         }
-        if (amax != amax) q[0] = q[1] = 0x7f7f7f7fu;
-        if (!live) continue;
-        ((u32x2*)(a.out + (int64_t)row * a.out_ld))[v] = u32x2{q[0], q[1]};
-        if ((lane & 15) == 0) a.sf[(int64_t)row * a.sf_row + (int64_t)(v >> 4) * a.sf_col] = kind == 2 ? amax / 448.0f : 0.0f;
     }
 }
 extern "C" __global__ __launch_bounds__(256) void ep_swiglu_bf16(EpSwigluArgs a) { swiglu_body<false>(a); }
@@ -956,7 +1148,8 @@ extern "C" __global__ __launch_bounds__(256) void ep_swiglu_gradients(EpSwigluAr
     const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
     const int64_t task = (int64_t)blockIdx.x * 4 + wave;
     if (task >= a.layout.num_rows) return;
-    const int row = (int)task, kind = kind_of_row(a.layout, row);
+    int expert;
+    const int row = (int)task, kind = kind_of_row(a.layout, row, expert);
     if (kind == 0) return;
     const float weight = kind == 2 && a.weights != nullptr ? a.weights[row] : 1.0f;
     const u32x4* const h = (const u32x4*)(a.h + (int64_t)row * a.h_ld * 2);
@@ -968,9 +1161,9 @@ extern "C" __global__ __launch_bounds__(256) void ep_swiglu_gradients(EpSwigluAr
         float of_gate[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, of_up[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (kind == 2) {
             float gate[8], up[8], grad[8];
-            widen(h[v], gate);
-            widen(h[vectors + v], up);
-            widen(grad_out[v], grad);
+            widen(__builtin_nontemporal_load(h + v), gate);
+            widen(__builtin_nontemporal_load(h + vectors + v), up);
+            widen(__builtin_nontemporal_load(grad_out + v), grad);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float s = sigmoid(gate[i]), silu = gate[i] * s;
@@ -980,8 +1173,8 @@ extern "C" __global__ __launch_bounds__(256) void ep_swiglu_gradients(EpSwigluAr
                 of_gate[i] = g * up[i] * s * (1.0f + gate[i] * (1.0f - s));
             }
         }
-        grad_h[v] = round_bf16(of_gate);
-        grad_h[vectors + v] = round_bf16(of_up);
+        store<true>(grad_h + v, round_bf16(of_gate));
+        store<true>(grad_h + vectors + v, round_bf16(of_up));
     }
     if (a.grad_weights == nullptr) return;
 #pragma unroll

@@ -619,7 +619,7 @@ at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const O
 
 at::Tensor linear_workspace(ep_grouped_linear_args_t& a, const at::Device& device) {
     if (a.transpose_weight) return {};
-    a.workspace_bytes = ep_grouped_linear_workspace_bytes(a.x.size[0], a.num_experts, a.expert_alignment, a.x.size[1], a.weight.size[0], a.x.dtype);
+    a.workspace_bytes = ep_grouped_linear_workspace_bytes(a.x.size[0], a.num_experts, a.expert_alignment, a.x.size[1], a.weight.size[0]);
     if (a.workspace_bytes == 0) return {};
     const at::Tensor workspace = alloc({a.workspace_bytes}, at::kByte, device);
     a.workspace = workspace.data_ptr();

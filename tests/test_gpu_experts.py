@@ -136,8 +136,8 @@ def test_depth_in_parts(counts, alignment, depth, columns, kind):
     """Few tiles: the depth is split, the parts are added in a launch of their own."""
     layout = U.Layout(counts, alignment, tail=3)
     experts = len(counts)
-    assert deep_ep._C._lib.ep_grouped_linear_workspace_bytes(layout.rows, experts, alignment, deep_ep._C.ctypes.c_int64(depth),
-                                                             deep_ep._C.ctypes.c_int64(columns), 2 if kind == 'fp8' else 1) > 0
+    assert deep_ep._C._lib.ep_grouped_linear_workspace_bytes(deep_ep._C.ctypes.c_int64(layout.rows), experts, alignment, deep_ep._C.ctypes.c_int64(depth),
+                                                             deep_ep._C.ctypes.c_int64(columns)) > 0
     x, w = U.normal(1, layout.rows, depth), U.normal(2, experts, columns, depth, scale=depth ** -0.5)
     a, b = U.normal(4, 3, experts, 8, depth, scale=depth ** -0.5), U.normal(5, 3, experts, columns, 8)
     idx = (torch.arange(layout.rows) % 4 - 1).to(torch.int32)

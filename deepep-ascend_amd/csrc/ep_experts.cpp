@@ -14,14 +14,14 @@ struct Tile {
     int rows, columns, threads;
 };
 constexpr Tile kTiles[] = {{32, 64, 256}, {64, 128, 256}, {64, 256, 512}, {128, 256, 512}, {256, 256, 512}};
-constexpr int kNumTiles = 5, kTile32 = 0, kTile64 = 1, kTile64Wide = 2, kTile128 = 3, kTile256 = 4;
+enum { kTile32, kTile64, kTile64Wide, kTile128, kTile256, kNumTiles };
 constexpr int kKindBf16 = 0, kKindFp8 = 1, kKindLora = 2, kKindTransposed = 3;
 
 struct ExpertKernels {
     hipModule_t module = nullptr;
     int device = -1;
     hipFunction_t rows[4][kNumTiles];             // [kKind*][kTiles]
-    hipFunction_t split[2], split_lora[3], sum_splits, sum_splits_lora;
+    hipFunction_t split[2], split_lora[3], sum_splits, sum_splits_lora, split_weights, sum_weights[2];
     hipFunction_t weights[2][2];                  // [BF16, float32][128 x 128, 256 x 256]
     hipFunction_t swiglu[2], swiglu_grad, lora_down[3], lora_down_rows, expand_fill, expand_rows;
 };
@@ -91,21 +91,53 @@ int64_t mean_rows(int64_t rows, int num_experts, int alignment) {
 struct Plan {
     int tile, splits, split_depth;
 };
+// Rounds of the chip's 256 CUs times what a round takes, in hundredths of one of 256 x 256 tiles.  Measured in us, BF16, tiles of 64 x 128
+// (two workgroups a CU) / 64 x 256 / 128 x 256 / 256 x 256:
+//   one expert, 7168 channels to 2048, 1500 rows 94 61 75 126, 3000 rows 115 125 84 130, 6000 rows 228 197 166 140, 12000 rows 444 385 277 296
+//   8 experts, 4096 to 2048, 1500 rows 50 41 48 77, 3000 84 74 51 76, 6000 151 143 100 86, 12000 341 273 207 172, 16384 416 398 275 261
+//   64 experts, 2560 to 1536, 7147 rows 162 160 124 121, of Zipf(0.6) popularity 161 163 146 131
+//   32 experts, 4096 to 4096, 3500 rows 309 240 199 281, 6000 rows 521 456 257 311
+// (the last two are bound by the weights).  Experts end inside a tile, half of one on average.
 Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool transposed) {
     const int64_t mean = mean_rows(rows, num_experts, alignment);
-    const auto tiles = [&](int t) { return row_tiles_bound(rows, num_experts, kTiles[t].rows) * ceil_div(columns, kTiles[t].columns); };
-    Plan p{mean <= 64 ? kTile128 : kTile256, 1, 0};
-    if (transposed) return p;
-    if (mean <= 40) p.tile = tiles(kTile64Wide) <= 256 ? kTile64 : kTile64Wide;
-    if (p.tile == kTile64 or rows <= 1024) {
-        const int64_t steps = ceil_div(depth, 128), few = tiles(kTile64);
-        if (few < 256) {
-            p.splits = (int)std::clamp<int64_t>(512 / few, 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
-            p.split_depth = (int)(ceil_div(steps, p.splits) * 128);
-            p.splits = (int)ceil_div(depth, p.split_depth);
-            p.tile = p.splits > 1 ? kTile64 : kTile32;
+    const int64_t cost[kNumTiles] = {0, 55, 48, 62, 100}, slots[kNumTiles] = {512, 512, 256, 256, 256};
+    int64_t tiles[kNumTiles], best = INT64_MAX;
+    Plan p{kTile256, 1, 0};
+    for (int t = kTile64; t < kNumTiles; ++t) {
+        const int64_t high = kTiles[t].rows, wide = ceil_div(columns, kTiles[t].columns);
+        tiles[t] = num_experts == 1 ? ceil_div(rows, high) * wide : std::max<int64_t>(num_experts, num_experts * (2 * mean + high) / (2 * high)) * wide;
+        const int64_t time = ceil_div(tiles[t], slots[t]) * cost[t];
+        // (of equals the larger tile where its rows are there, the smaller where they are not)
+        if (time < best or (time == best and mean > 64)) {
+            best = time;
+            p.tile = t;
         }
     }
+    // half a round of wide tiles: as many bytes of weights in flight with twice the workgroups (32 experts of 8 rows, 4096 channels to 2048,
+    // 122 -> 108 us)
+    if (p.tile == kTile64Wide and tiles[kTile64Wide] <= 256) p.tile = kTile64;
+    if (transposed) return p;
+    if (tiles[kTile64] < 256) {
+        const int64_t steps = ceil_div(depth, 128);
+        p.splits = (int)std::clamp<int64_t>(512 / tiles[kTile64], 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
+        p.split_depth = (int)(ceil_div(steps, p.splits) * 128);
+        p.splits = (int)ceil_div(depth, p.split_depth);
+        p.tile = p.splits > 1 ? kTile64 : kTile32;
+    }
+    return p;
+}
+
+// The gradient of weights: tiles of 256 x 256 as soon as they fill the chip; where those of 128 x 128 do not either and rows are many, rows
+// in parts.
+struct WeightsPlan {
+    bool large;
+    int splits;
+};
+WeightsPlan plan_weights(int64_t rows, int num_experts, int alignment, int64_t out_rows, int64_t out_columns) {
+    WeightsPlan p{num_experts * ceil_div(out_rows, 256) * ceil_div(out_columns, 256) >= 256, 1};
+    const int64_t tiles = num_experts * ceil_div(out_rows, 128) * ceil_div(out_columns, 128);
+    if (not p.large and tiles < 256)
+        p.splits = (int)std::clamp<int64_t>(512 / tiles, 1, std::clamp<int64_t>(mean_rows(rows, num_experts, alignment) / 512, 1, 32));
     return p;
 }
 
@@ -125,13 +157,16 @@ void ep_load_expert_kernels(const char* dir) {
     const char* kinds[] = {"bf16", "fp8", "lora", "transposed"};
     for (int k = 0; k < 4; ++k) {
         for (int t = 0; t < kNumTiles; ++t) {
-            if (k == kKindTransposed and t < kTile128) continue;
+            if (k == kKindTransposed and t == kTile32) continue;
             get(g_k.rows[k][t], format("ep_grouped_%s_%dx%d", kinds[k], kTiles[t].rows, kTiles[t].columns).c_str());
         }
     }
     for (int k = 0; k < 2; ++k) get(g_k.split[k], format("ep_grouped_split_%s", kinds[k]).c_str());
     for (int i = 0; i < 3; ++i) get(g_k.split_lora[i], format("ep_grouped_split_lora_%d", 16 << i).c_str());
     get(g_k.sum_splits, "ep_sum_splits");
+    get(g_k.split_weights, "ep_grouped_split_weights");
+    get(g_k.sum_weights[0], "ep_sum_weights_bf16");
+    get(g_k.sum_weights[1], "ep_sum_weights_f32");
     get(g_k.sum_splits_lora, "ep_sum_splits_lora");
     for (int i = 0; i < 3; ++i) get(g_k.lora_down[i], format("ep_lora_down_16_%d", 16 << i).c_str());
     get(g_k.lora_down_rows, "ep_lora_down_rows");
@@ -222,22 +257,20 @@ static void launch_rows(EpGemmArgs& g, int kind, const LoraPlan* lora, void* wor
     g.column_tiles = (int)ceil_div(g.num_columns, t.columns);
     g.splits = p.splits;
     g.split_depth = p.split_depth;
-    g.partial = (float*)workspace;
+    g.partial = p.splits > 1 ? (float*)workspace : nullptr;
     const int64_t row_tiles = row_tiles_bound(l.num_rows, l.num_experts, t.rows);
     EP_HOST_ASSERT(row_tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles * p.splits));
     const int64_t blocks = align_up(row_tiles * g.column_tiles * p.splits, 8);
     const int ranks = g.lora.rank <= 16 ? 0 : g.lora.rank <= 32 ? 1 : 2;
+    // (few rows' low-rank rows come with the parts of the product, in one launch)
+    const bool together = lora != nullptr and lora->rows == 16 and p.splits > 1;
+    if (lora != nullptr and not together) launch(lora->rows == 16 ? k.lora_down[ranks] : k.lora_down_rows, g.lora.blocks, 256, stream, g);
     if (p.splits == 1) {
-        if (lora != nullptr) launch(lora->rows == 16 ? k.lora_down[ranks] : k.lora_down_rows, g.lora.blocks, 256, stream, g);
         launch(k.rows[kind][p.tile], blocks, t.threads, stream, g);
         return;
     }
-    if (lora != nullptr) {
-        EP_HOST_ASSERT(lora->rows == 16);
-        launch(k.split_lora[ranks], g.lora.blocks + blocks, t.threads, stream, g);
-    } else {
-        launch(k.split[kind], blocks, t.threads, stream, g);
-    }
+    if (together) launch(k.split_lora[ranks], g.lora.blocks + blocks, t.threads, stream, g);
+    else launch(k.split[kind == kKindFp8 ? 1 : 0], blocks, t.threads, stream, g);
     launch(lora != nullptr ? k.sum_splits_lora : k.sum_splits, ceil_div((int64_t)l.num_rows * ceil_div(g.num_columns, 512), 4), 256, stream, g);
 }
 
@@ -344,6 +377,8 @@ int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
     return guarded([&] {
         EP_HOST_ASSERT(args != nullptr);
         const ep_tensor_t &grad = args->grad, &x = args->x, &out = args->out;
+        EP_HOST_ASSERT(args->workspace_bytes >= 0 and (args->workspace != nullptr or args->workspace_bytes == 0));
+        EP_HOST_ASSERT(((uintptr_t)args->workspace & 15) == 0);
         EP_HOST_ASSERT(row_major(grad) and grad.dtype == EP_DTYPE_BF16 and addressable(grad));
         EP_HOST_ASSERT(row_major(x) and x.dtype == EP_DTYPE_BF16 and addressable(x));
         EP_HOST_ASSERT(x.size[0] == grad.size[0] and x.size[1] % 8 == 0 and grad.size[1] % 8 == 0);
@@ -364,17 +399,31 @@ int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
         g.out_expert = args->out_expert_stride;
         g.num_columns = (int)x.size[1];
         g.num_out_rows = (int)grad.size[1];
-        // (tiles of 256 x 256 as soon as they fill the chip)
-        const bool large = (int64_t)g.layout.num_experts * ceil_div(g.num_columns, 256) * ceil_div(g.num_out_rows, 256) >= 256;
-        const int tile = large ? 256 : 128;
+        const int experts = g.layout.num_experts;
+        WeightsPlan p = plan_weights(g.layout.num_rows, experts, g.layout.alignment, g.num_out_rows, g.num_columns);
+        const int64_t bytes = (int64_t)p.splits * experts * g.num_out_rows * g.num_columns * 4;
+        if (p.splits > 1 and bytes > args->workspace_bytes) p.splits = 1;
+        const int tile = p.large ? 256 : 128;
         g.column_tiles = (int)ceil_div(g.num_columns, tile);
         g.row_tiles = (int)ceil_div(g.num_out_rows, tile);
+        g.splits = p.splits;
+        g.partial = p.splits > 1 ? (float*)args->workspace : nullptr;
         g.accumulate = args->accumulate != 0;
         g.few_rows = mean_rows(g.layout.num_rows, g.layout.num_experts, g.layout.alignment) <= 256;
-        const int64_t tiles = (int64_t)g.layout.num_experts * g.row_tiles;
+        const int64_t tiles = (int64_t)experts * g.row_tiles * p.splits;
         EP_HOST_ASSERT(tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles));
-        launch(kernels().weights[f32 ? 1 : 0][large ? 1 : 0], align_up(tiles * g.column_tiles, 8), 512, args->stream, g);
+        const ExpertKernels& k = kernels();
+        launch(p.splits > 1 ? k.split_weights : k.weights[f32 ? 1 : 0][p.large ? 1 : 0], align_up(tiles * g.column_tiles, 8), 512, args->stream, g);
+        if (p.splits > 1) launch(k.sum_weights[f32 ? 1 : 0], ceil_div((int64_t)experts * g.num_out_rows * g.num_columns, 1024), 256, args->stream, g);
     });
+}
+
+int64_t ep_grouped_weight_grad_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t out_rows, int64_t out_columns) {
+    if (num_rows <= 0 or num_rows > INT32_MAX or num_experts <= 0 or expert_alignment <= 0 or out_rows <= 0 or out_rows > INT32_MAX / 2 or
+        out_columns <= 0 or out_columns > INT32_MAX / 2)
+        return 0;
+    const WeightsPlan p = plan_weights(num_rows, num_experts, expert_alignment, out_rows, out_columns);
+    return p.splits > 1 ? (int64_t)p.splits * num_experts * out_rows * out_columns * 4 : 0;
 }
 
 static EpSwigluArgs swiglu_args(const ep_tensor_t& h, const ep_tensor_t& weights, const ep_tensor_t& psum, int num_experts, int alignment,

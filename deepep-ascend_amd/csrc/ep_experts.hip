@@ -225,10 +225,8 @@ struct TileFetch {
             return buffer_of(base + (int64_t)s * 64 * ld, rows > 0 ? (unsigned)((rows - 1) * ld) + bytes : 0u);
         }
         const int left = depth_bytes - s * 128;
-        if (left < 128) {
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) from[i] = chunk * 16 < left ? from[i] : OUTSIDE;
-        }
+        for (int i = 0; i < MINE; ++i) from[i] = chunk * 16 < left ? from[i] : OUTSIDE;
         return buffer_of(base + (int64_t)s * 128, left > 0 && bytes > 0 ? bytes - s * 128 : 0u);
     }
     __device__ __forceinline__ void fetch(i32x4 buffer, int i, unsigned to, int wave) const { fetch16(to + piece(i, wave) * 1024, from[i], buffer); }
@@ -416,14 +414,23 @@ struct Gemm {
             i32x4 columns, rows, sf;
             unsigned to_columns, to_rows, to_sf;
         };
+        // (in three shares: between the matrix instructions, the scalar unit's time does not show)
+        auto begin_share = [&](Fetches& f, int share, int s_rows, int slot_rows, int s_columns, int slot_columns) {
+            if (share == 0) {
+                f.rows = rf.step(s_rows);
+                f.to_rows = lds0 + ROWS_AT + slot_rows * ROWS_BYTES;
+            } else if (share == 1) {
+                f.columns = cf.step(s_columns);
+                f.to_columns = lds0 + slot_columns * COLUMNS_BYTES;
+            } else if (FP8) {
+                f.sf = buffer_of((const char*)(rows_sf + s_rows * a.rows_sf_col), s_rows < steps ? sf_bytes : 0u);
+                f.to_sf = lds0 + SF_AT + slot_rows * SF_BYTES + (wave % SF_PIECES) * 256;
+            }
+        };
         auto begin_fetch = [&](int s_rows, int slot_rows, int s_columns, int slot_columns) {
             Fetches f;
-            f.rows = rf.step(s_rows);
-            f.columns = cf.step(s_columns);
-            if (FP8) f.sf = buffer_of((const char*)(rows_sf + s_rows * a.rows_sf_col), s_rows < steps ? sf_bytes : 0u);
-            f.to_columns = lds0 + slot_columns * COLUMNS_BYTES;
-            f.to_rows = lds0 + ROWS_AT + slot_rows * ROWS_BYTES;
-            f.to_sf = lds0 + SF_AT + slot_rows * SF_BYTES + (wave % SF_PIECES) * 256;
+#pragma unroll
+            for (int share = 0; share < 3; ++share) begin_share(f, share, s_rows, slot_rows, s_columns, slot_columns);
             return f;
         };
         constexpr int OF_ROWS = RowsFetch::MINE + (FP8 ? 1 : 0);
@@ -492,9 +499,13 @@ struct Gemm {
                 for (int i = 0; i < READS; ++i) read_one(c[0], r[0], 0, 0, 0, i);
             }
             for (int s = 0; s < steps; ++s) {
+                Fetches f;
                 if (active) {
 #pragma unroll
                     for (int p = 0; p < PRODUCTS; ++p) {
+#pragma unroll
+                        for (int share = 0; share < 2; ++share)
+                            if (p == (share + 1) * PRODUCTS / 3) begin_share(f, share, s + SR, slot_rows, s + SC, slot_columns);
                         // (early: they have arrived before the wave waits for the others)
 #pragma unroll
                         for (int i = 0; i < READS; ++i)
@@ -503,7 +514,7 @@ struct Gemm {
                         KEEP_ORDER();
                     }
                 }
-                const Fetches f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
+                if (!active) f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
                 slot_rows = next(slot_rows, SR);
                 slot_columns = next(slot_columns, SC);
                 KEEP_ORDER();
@@ -590,13 +601,18 @@ struct Gemm {
 #pragma unroll
                         for (int p = 0; p < LAST; ++p) {
                             fetch_at(f, p + 2 * NC);
+                            // (the fetches in flight are done with `f`)
+                            constexpr int FROM = SPREAD - 2 * NC < LAST ? SPREAD - 2 * NC : LAST - 1;
+#pragma unroll
+                            for (int share = 0; share < 3; ++share)
+                                if (p == FROM + share * (LAST - FROM) / 3) begin_share(f, share, s + SR, slot_rows, s + SC, slot_columns);
                             if (p % NC == 0 && p / NC + 2 < NR) read_row(r[(p / NC + 2) % 4], scales[(p / NC + 2) % 4], slot_rows, p / NC + 2);
                             scale_one(p - DEPTH);
                             sums[p % DEPTH] = multiply(c[column_of(p)], r[row_of(p) % 4]);
                             KEEP_ORDER();
                         }
                     }
-                    f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
+                    if (!active) f = begin_fetch(s + SR, slot_rows, s + SC, slot_columns);
                     slot_rows = next(slot_rows, SR);
                     slot_columns = next(slot_columns, SC);
                     KEEP_ORDER();
@@ -683,7 +699,7 @@ struct Gemm {
                     *(f32x4*)((float*)out + (int64_t)r * a.lora.rank + (column - segment * a.lora.rank)) = __builtin_bit_cast(f32x4, v) * scale;
                     continue;
                 }
-                if (OUT32 && a.accumulate) {
+                if (OUT32 && a.accumulate && a.partial == nullptr) {
                     const f32x4 sum = *(const f32x4*)to + __builtin_bit_cast(f32x4, v);
                     v = __builtin_bit_cast(u32x4, sum);
                 }
@@ -805,24 +821,40 @@ struct Gemm {
     }
 
     // Gradient of an expert's weights: out[e][r, c] = sum over the expert's rows d of rows[d, r] columns[d, c]
+    // SPLIT: of a part of the expert's rows; ep_sum_weights adds the parts.
+    template <bool SPLIT>
     __device__ __forceinline__ static void weights_kernel(const EpGemmArgs& a, int group) {
-        int row, column;
-        const int row_tiles = a.row_tiles * a.layout.num_experts;
+        int row, column, part = 0;
+        const int row_tiles = a.row_tiles * a.layout.num_experts, column_tiles = SPLIT ? a.column_tiles * a.splits : a.column_tiles;
         if (a.few_rows) {
             // the time is the results': the tiles of an expert with many rows go to all XCDs
-            if ((int)blockIdx.x >= row_tiles * a.column_tiles) return;
-            row = blockIdx.x / a.column_tiles;
-            column = blockIdx.x - row * a.column_tiles;
-        } else if (!tile_of_block(blockIdx.x, row_tiles, a.column_tiles, group, row, column)) {
+            if ((int)blockIdx.x >= row_tiles * column_tiles) return;
+            row = blockIdx.x / column_tiles;
+            column = blockIdx.x - row * column_tiles;
+        } else if (!tile_of_block(blockIdx.x, row_tiles, column_tiles, group, row, column)) {
             return;
+        }
+        if (SPLIT) {
+            part = column % a.splits;
+            column /= a.splits;
         }
         const int e = row / a.row_tiles, r0 = (row - e * a.row_tiles) * TM, c0 = column * TN;
         const ExpertRows in = rows_of_expert(a.layout, e);
-        const int count = uniform(in.count);
-        const int64_t start = uniform(in.start);
+        int count = uniform(in.count);
+        int64_t start = uniform(in.start);
+        char* out = a.out;
+        int64_t out_expert = a.out_expert, out_ld = a.out_ld;
+        if (SPLIT) {
+            const int share = align_up(ceil_div(count, a.splits), STEP), from = min(part * share, count);
+            start += from;
+            count = min(count - from, share);
+            out_ld = a.num_columns;
+            out_expert = (int64_t)a.num_out_rows * out_ld;
+            out = (char*)(a.partial + (int64_t)part * a.layout.num_experts * out_expert);
+        }
         const int out_rows = min(a.num_out_rows - r0, TM);
         run(a, a.rows + start * a.rows_ld + (int64_t)r0 * 2, a.columns + start * a.columns_ld + (int64_t)c0 * 2, out_rows, out_rows,
-            a.num_columns - c0, count, nullptr, nullptr, a.out + (e * a.out_expert + (int64_t)r0 * a.out_ld + c0) * OUT_ELEM, a.out_ld);
+            a.num_columns - c0, count, nullptr, nullptr, out + (e * out_expert + (int64_t)r0 * out_ld + c0) * OUT_ELEM, out_ld);
     }
 };
 
@@ -838,9 +870,9 @@ extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_fp8(EpGemmArg
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
         Gemm<TM, TN, WR, WC, MT, SR, SC, false, false, false, false, true>::rows_kernel<false>(a, GROUP);             \
     }
-#define EP_GEMM_WEIGHTS(NAME, TM, TN, WR, WC, MT, SR, SC, OUT32, GROUP)                                               \
+#define EP_GEMM_WEIGHTS(NAME, TM, TN, WR, WC, MT, SR, SC, OUT32, SPLIT, GROUP)                                        \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, MT, SR, SC, false, true, true, OUT32>::weights_kernel(a, GROUP);                         \
+        Gemm<TM, TN, WR, WC, MT, SR, SC, false, true, true, OUT32>::weights_kernel<SPLIT>(a, GROUP);                         \
     }
 EP_GEMM_ROWS(ep_grouped_bf16_32x64, 32, 64, 1, 4, 16, 4, 4, false, false, 4)
 EP_GEMM_ROWS(ep_grouped_bf16_64x128, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
@@ -852,6 +884,8 @@ EP_GEMM_ROWS(ep_grouped_fp8_64x128, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
 EP_GEMM_ROWS(ep_grouped_fp8_64x256, 64, 256, 1, 8, 16, 3, 3, true, false, 1)
 EP_GEMM_ROWS(ep_grouped_fp8_128x256, 128, 256, 2, 4, 16, 3, 3, true, false, 1)
 EP_GEMM_ROWS(ep_grouped_fp8_256x256, 256, 256, 2, 4, 16, 2, 2, true, false, 8)
+EP_GEMM_ROWS(ep_grouped_transposed_64x128, 64, 128, 2, 2, 16, 3, 3, false, true, 1)
+EP_GEMM_ROWS(ep_grouped_transposed_64x256, 64, 256, 1, 8, 16, 3, 3, false, true, 1)
 EP_GEMM_ROWS(ep_grouped_transposed_128x256, 128, 256, 2, 4, 16, 3, 3, false, true, 1)
 EP_GEMM_ROWS(ep_grouped_transposed_256x256, 256, 256, 2, 4, 16, 2, 3, false, true, 8)
 EP_GEMM_LORA(ep_grouped_lora_32x64, 32, 64, 1, 4, 16, 4, 4, 4)
@@ -859,10 +893,11 @@ EP_GEMM_LORA(ep_grouped_lora_64x128, 64, 128, 2, 2, 16, 3, 3, 1)
 EP_GEMM_LORA(ep_grouped_lora_64x256, 64, 256, 1, 8, 16, 3, 3, 1)
 EP_GEMM_LORA(ep_grouped_lora_128x256, 128, 256, 2, 4, 16, 3, 3, 1)
 EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 16, 2, 3, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 2, 2, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 16, 2, 3, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 2, 2, true, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 16, 2, 3, true, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 2, 2, false, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 16, 2, 3, false, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 2, 2, true, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 16, 2, 3, true, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_split_weights, 128, 128, 2, 4, 16, 2, 2, true, true, 8)
 
 // ---- low-rank adapters: rows times the first matrix ---------------------------------------------------------
 //
@@ -1004,7 +1039,7 @@ extern "C" __global__ __launch_bounds__(256) void ep_expand_token_index_rows(EpE
 
 // ---- parts of a depth, added -----------------------------------------------------------------------------
 
-// A lane has eight columns of a row, and adds what the row's adapter makes of its low-rank row.
+// Of rows: a lane has eight columns of one, and adds what the row's adapter makes of its low-rank row.
 template <bool LORA>
 __device__ __forceinline__ void sum_splits_body(const EpGemmArgs& a) {
     const int vectors = a.num_columns >> 3, per_row = ceil_div(vectors, WAVE);
@@ -1050,6 +1085,27 @@ __device__ __forceinline__ void sum_splits_body(const EpGemmArgs& a) {
     for (int i = 0; i < 8; ++i) out[i] = (__bf16)sum[i >> 2][i & 3];
     *((bf16x8*)(a.out + row * a.out_ld * 2) + v) = out;
 }
+// Parts of an expert's rows: a lane has four weights.
+template <bool OUT32>
+__device__ __forceinline__ void sum_weights_body(const EpGemmArgs& a) {
+    const int64_t of_expert = (int64_t)a.num_out_rows * a.num_columns, all = of_expert * a.layout.num_experts;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= all) return;
+    f32x4 sum = {};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) sum += *(const f32x4*)(a.partial + s * all + at);
+    const int64_t e = at / of_expert, in = at - e * of_expert, r = in / a.num_columns, c = in - r * a.num_columns;
+    const int64_t to = e * a.out_expert + r * a.out_ld + c;
+    if (OUT32) {
+        f32x4* const out = (f32x4*)((float*)a.out + to);
+        *out = a.accumulate ? *out + sum : sum;
+    } else {
+        *(bf16x4*)((__bf16*)a.out + to) = __builtin_convertvector(sum, bf16x4);
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void ep_sum_weights_bf16(EpGemmArgs a) { sum_weights_body<false>(a); }
+extern "C" __global__ __launch_bounds__(256) void ep_sum_weights_f32(EpGemmArgs a) { sum_weights_body<true>(a); }
+
 extern "C" __global__ __launch_bounds__(256) void ep_sum_splits(EpGemmArgs a) { sum_splits_body<false>(a); }
 extern "C" __global__ __launch_bounds__(256) void ep_sum_splits_lora(EpGemmArgs a) { sum_splits_body<true>(a); }
 

@@ -698,6 +698,12 @@ at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, cons
     a.num_experts = num_experts;
     a.expert_alignment = alignment;
     a.accumulate = accumulate;
+    a.workspace_bytes = ep_grouped_weight_grad_workspace_bytes(x.size(0), num_experts, alignment, grad.size(1), x.size(1));
+    at::Tensor workspace;
+    if (a.workspace_bytes > 0) {
+        workspace = alloc({a.workspace_bytes}, at::kByte, x.device());
+        a.workspace = workspace.data_ptr();
+    }
     a.stream = current_stream();
     check(ep_grouped_weight_grad(&a));
     return w;

@@ -378,8 +378,11 @@ typedef struct ep_grouped_weight_grad_args {
     int64_t out_expert_stride;          /* elements */
     int32_t num_experts, expert_alignment;
     int32_t accumulate;                 /* fp32: added to what is there */
+    void* workspace;                    /* of the call's own, or NULL: with ep_grouped_weight_grad_workspace_bytes bytes the rows of few */
+    int64_t workspace_bytes;            /* and small matrices are split */
     void* stream;
 } ep_grouped_weight_grad_args_t;
+int64_t ep_grouped_weight_grad_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t out_rows, int64_t out_columns);
 /* out[e] = sum over the rows m of expert e of grad[m] x[m]^T; zeros for an expert without rows. */
 int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args);
 

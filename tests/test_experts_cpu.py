@@ -32,7 +32,8 @@ class Linear(ctypes.Structure):
 
 class WeightGrad(ctypes.Structure):
     _fields_ = [(n, Tensor) for n in ('grad', 'x', 'psum', 'out')] + [('out_expert_stride', ctypes.c_int64)] + [
-        (n, ctypes.c_int32) for n in ('num_experts', 'expert_alignment', 'accumulate')] + [('stream', ctypes.c_void_p)]
+        (n, ctypes.c_int32) for n in ('num_experts', 'expert_alignment', 'accumulate')] + [
+        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64), ('stream', ctypes.c_void_p)]
 
 
 class Swiglu(ctypes.Structure):
@@ -135,7 +136,8 @@ def test_grouped_linear_of_fp8_refuses(lib, case):
 
 @pytest.mark.parametrize('change', [
     dict(x=matrix(63, 256)), dict(grad=matrix(64, 128, FP8)), dict(grad=matrix(64, 124, ld=128)), dict(out=matrix(128, 248, ld=256)),
-    dict(out=matrix(128, 256, 5)), dict(accumulate=1), dict(out_expert_stride=128 * 256 - 8), dict(num_experts=3), dict(psum=Tensor())])
+    dict(out=matrix(128, 256, 5)), dict(accumulate=1), dict(out_expert_stride=128 * 256 - 8), dict(num_experts=3), dict(psum=Tensor()),
+    dict(workspace_bytes=64), dict(workspace=4100, workspace_bytes=64), dict(workspace=4096, workspace_bytes=-4)])
 def test_grouped_weight_grad_refuses(lib, change):
     a = WeightGrad()
     values = dict(grad=matrix(64, 128), x=matrix(64, 256), psum=vector(4, I32), out=matrix(128, 256), out_expert_stride=128 * 256,

@@ -98,7 +98,8 @@ def test_grouped_linear_gradients(name, depth, columns):
 
 
 # mean rows of an expert on both sides of the lines between tiles, tails of every size in them
-@pytest.mark.parametrize('counts', [[700, 0, 190, 513], [257, 383, 128, 64, 1], [160, 161, 90], [40, 47, 48, 49, 16], [5000]])
+@pytest.mark.parametrize('counts', [[700, 0, 190, 513], [257, 383, 128, 64, 1], [160, 161, 90], [40, 47, 48, 49, 16], [5000], [9000, 9100, 7],
+                                    [97] * 40, [3, 80, 1, 0] * 40])
 @pytest.mark.parametrize('depth,columns', [(16, 520), (1008, 776), (2048, 256)])
 @pytest.mark.parametrize('kind', ['bf16', 'fp8', 'lora', 'gradients'])
 def test_every_tile(counts, depth, columns, kind):
@@ -160,6 +161,27 @@ def test_depth_in_parts(counts, alignment, depth, columns, kind):
             deep_ep.grouped_linear(_dev(x), _dev(w), layout.on(DEV), out=out, do_zero_padding=zeroed)
         U.assert_sum(out[v.to(DEV)], want[v], size[v], depth, more=more[v])
         _check_rows(out, layout, zeroed, 77.0)
+
+
+@pytest.mark.parametrize('counts', [[5000], [2100, 0, 1700]])
+@pytest.mark.parametrize('rows,columns', [(72, 136), (256, 512)])
+def test_weight_gradients_of_rows_in_parts(counts, rows, columns):
+    layout = U.Layout(counts, 16)
+    experts = len(counts)
+    lib, c64 = deep_ep._C._lib, deep_ep._C.ctypes.c_int64
+    assert lib.ep_grouped_weight_grad_workspace_bytes(c64(layout.rows), experts, 16, c64(rows), c64(columns)) > 0
+    grad, x = U.spoil(U.normal(1, layout.rows, rows), layout), U.spoil(U.normal(2, layout.rows, columns), layout)
+    w = torch.zeros(experts, rows, columns, dtype=torch.bfloat16, device=DEV)
+    want, size = U.weight_grad(torch.nan_to_num(grad), torch.nan_to_num(x), layout)
+    _, gw = deep_ep.grouped_linear_grad(_dev(grad), _dev(x), w, layout.on(DEV), need_x=False)
+    U.assert_sum(gw, want, size, max(counts))
+    held = U.normal(4, experts, rows, columns).float()
+    wide = torch.zeros(experts, rows + 8, columns + 8, device=DEV)
+    total = wide[:, 8:, 8:]
+    total.copy_(held)
+    deep_ep.grouped_linear_grad(_dev(grad), _dev(x), w, layout.on(DEV), need_x=False, grad_weight=total, accumulate=True)
+    U.assert_sum(total, want + held.double(), size + held.double().abs(), max(counts), half=2.0 ** -24)
+    assert (wide[:, :8] == 0).all() and (wide[:, :, :8] == 0).all()
 
 
 def test_gradients_agree_with_differences():

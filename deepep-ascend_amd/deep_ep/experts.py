@@ -30,8 +30,6 @@ from .buffers.ep import EPHandle
 _native = _C._native
 _Layout = Union[EPHandle, Tuple[torch.Tensor, int], None]
 _TensorOrPair = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
-# what is written into rows of no expert besides nothing (0) and zeros in the padding (1): a gradient is zero there, all of it
-_ZERO_ALL = 2
 
 
 def _layout(layout: _Layout) -> Tuple[Optional[torch.Tensor], int]:
@@ -47,31 +45,8 @@ def _pair(x: _TensorOrPair) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     return x if isinstance(x, tuple) else (x, None)
 
 
-def _rows(grad: torch.Tensor) -> torch.Tensor:
-    """A gradient as the kernels address it: autograd also hands out broadcast and transposed ones."""
-    ok = grad.stride(1) == 1 and (grad.size(0) <= 1 or (grad.stride(0) >= grad.size(1) and grad.stride(0) % 8 == 0)) \
-        and grad.data_ptr() % 16 == 0
-    return grad if ok else grad.clone(memory_format=torch.contiguous_format)
-
-
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _GroupedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, psum, alignment, do_zero_padding):
-        ctx.save_for_backward(x, weight, psum)
-        ctx.alignment = alignment
-        return _native.grouped_linear(x, None, weight, None, psum, alignment, None, do_zero_padding, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, psum = ctx.saved_tensors
-        layout = None if psum is None else (psum, ctx.alignment)
-        grad_x, grad_weight = _grouped_linear_grad(grad, x, weight, layout, ctx.needs_input_grad[0], ctx.needs_input_grad[1], _ZERO_ALL)
-        return grad_x, grad_weight, None, None, None
 
 
 def grouped_linear(x: _TensorOrPair, weight: _TensorOrPair, layout: _Layout = None, *, out: Optional[torch.Tensor] = None,
@@ -94,7 +69,7 @@ def grouped_linear(x: _TensorOrPair, weight: _TensorOrPair, layout: _Layout = No
     if _wants_grad(x, weight, x_sf, weight_sf):
         if out is not None or x_sf is not None or weight_sf is not None:
             raise AssertionError('gradients are implemented for bfloat16 and without `out`')
-        return _GroupedLinear.apply(x, weight, psum, alignment, do_zero_padding)
+        return _native.grouped_linear_autograd(x, weight, psum, alignment, do_zero_padding)
     return _native.grouped_linear(x, x_sf, weight, weight_sf, psum, alignment, out, do_zero_padding, False)
 
 
@@ -109,13 +84,9 @@ def grouped_linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
         grad_weight: a tensor like `weight`, bfloat16 or float32, to store the weights' gradient into.
         accumulate: add to what `grad_weight` (float32) holds instead.
     """
-    return _grouped_linear_grad(grad, x, weight, layout, need_x, need_weight, int(do_zero_padding), grad_weight, accumulate)
-
-
-def _grouped_linear_grad(grad, x, weight, layout, need_x, need_weight, zero_rows, grad_weight=None, accumulate=False):
     psum, alignment = _layout(layout)
-    grad = _rows(grad)
-    grad_x = _native.grouped_linear(grad, None, weight, None, psum, alignment, None, zero_rows, True) if need_x else None
+    grad = _native.rows_of(grad)
+    grad_x = _native.grouped_linear(grad, None, weight, None, psum, alignment, None, do_zero_padding, True) if need_x else None
     if not need_weight:
         return grad_x, None
     if grad_weight is None:
@@ -123,20 +94,6 @@ def _grouped_linear_grad(grad, x, weight, layout, need_x, need_weight, zero_rows
         grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
     assert grad_weight.shape == weight.shape
     return grad_x, _native.grouped_weight_grad(grad, x, psum, weight.size(0) if weight.dim() == 3 else 1, alignment, grad_weight, accumulate)
-
-
-class _Swiglu(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, weights, psum, alignment, do_zero_padding):
-        ctx.save_for_backward(h, weights, psum)
-        ctx.alignment = alignment
-        return _native.swiglu(h, weights, psum, _num_experts(psum), alignment, False, None, None, do_zero_padding)[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        h, weights, psum = ctx.saved_tensors
-        return (*_native.swiglu_grad(_rows(grad), h, weights, psum, _num_experts(psum), ctx.alignment, _ZERO_ALL), None, None, None)
 
 
 def _num_experts(psum: Optional[torch.Tensor]) -> int:
@@ -163,7 +120,7 @@ def swiglu(h: torch.Tensor, layout: _Layout = None, topk_weights: Optional[torch
     if _wants_grad(h, topk_weights):
         if out is not None or fused_fp8_quant:
             raise AssertionError('gradients are implemented for bfloat16 and without `out`')
-        return _Swiglu.apply(h, topk_weights, psum, alignment, do_zero_padding)
+        return _native.swiglu_autograd(h, topk_weights, psum, _num_experts(psum), alignment, do_zero_padding)
     result, sf = _native.swiglu(h, topk_weights, psum, _num_experts(psum), alignment, fused_fp8_quant, out, out_sf, do_zero_padding)
     return (result, sf) if fused_fp8_quant else result
 
@@ -172,7 +129,7 @@ def swiglu_grad(grad: torch.Tensor, h: torch.Tensor, layout: _Layout = None, top
                 do_zero_padding: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of `swiglu` without autograd: `(grad_h [rows, 2 * I] bfloat16, grad_topk_weights [rows] float32` or None `)`."""
     psum, alignment = _layout(layout)
-    return _native.swiglu_grad(_rows(grad), h, topk_weights, psum, _num_experts(psum), alignment, do_zero_padding)
+    return _native.swiglu_grad(_native.rows_of(grad), h, topk_weights, psum, _num_experts(psum), alignment, do_zero_padding)
 
 
 def grouped_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_idx: torch.Tensor,

@@ -417,6 +417,43 @@ def test_broadcast_gradients():
     assert torch.equal(h.grad, deep_ep.swiglu_grad(torch.ones_like(a), h.detach(), layout.on(DEV), do_zero_padding=True)[0])
 
 
+def test_gradients_of_some_arguments_only():
+    layout = U.Layout([5, 20], 8)
+    x, w, h, g = _dev(U.normal(1, layout.rows, 64)), _dev(U.normal(2, 2, 32, 64)), _dev(U.normal(3, layout.rows, 64)), torch.rand(layout.rows, device=DEV)
+    grad = _dev(U.normal(4, layout.rows, 32))
+    gx, gw = deep_ep.grouped_linear_grad(grad, x, w, layout.on(DEV), do_zero_padding=True)
+    for with_x in (True, False):
+        lx, lw = x.detach().requires_grad_(with_x), w.detach().requires_grad_(not with_x)
+        deep_ep.grouped_linear(lx, lw, layout.on(DEV)).backward(grad)
+        assert torch.equal(lx.grad, gx) and lw.grad is None if with_x else torch.equal(lw.grad, gw) and lx.grad is None
+    gh, gg = deep_ep.swiglu_grad(grad, h, layout.on(DEV), g, do_zero_padding=True)
+    for with_h in (True, False):
+        lh, lg = h.detach().requires_grad_(with_h), g.detach().requires_grad_(not with_h)
+        deep_ep.swiglu(lh, layout.on(DEV), lg).backward(grad)
+        assert torch.equal(lh.grad, gh) and lg.grad is None if with_h else torch.equal(lg.grad, gg) and lh.grad is None
+
+
+def test_gradients_are_not_differentiated():
+    x, w = _dev(U.normal(1, 8, 64)).requires_grad_(), _dev(U.normal(2, 32, 64)).requires_grad_()
+    y = deep_ep.grouped_linear(x, w)
+    gx, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match='cannot be differentiated'):
+        gx.float().pow(2).sum().backward()
+    h = _dev(U.normal(3, 8, 64)).requires_grad_()
+    gh, = torch.autograd.grad(deep_ep.swiglu(h).sum(), h, create_graph=True)
+    with pytest.raises(RuntimeError, match='cannot be differentiated'):
+        gh.float().pow(2).sum().backward()
+
+
+def test_arguments_changed_before_the_backward_pass_are_noticed():
+    x, w = _dev(U.normal(1, 8, 64)).requires_grad_(), _dev(U.normal(2, 32, 64)).requires_grad_()
+    y = deep_ep.grouped_linear(x, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
 # ---- together, as they are used -----------------------------------------------------------------------------
 
 def _moe(tokens, hidden, inner, experts, topk, alignment, seed=0):

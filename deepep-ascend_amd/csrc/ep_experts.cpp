@@ -61,7 +61,7 @@ bool addressable(const ep_tensor_t& t) { return row_stride(t) * elem_size(t.dtyp
 EpExpertLayout layout_of(const ep_tensor_t& psum, int num_experts, int alignment, int zero_rows, int64_t rows) {
     EP_HOST_ASSERT(num_experts > 0 and alignment > 0);
     EP_HOST_ASSERT(zero_rows >= EP_ZERO_NONE and zero_rows <= EP_ZERO_ALL);
-    EP_HOST_ASSERT(rows + alignment <= INT32_MAX);
+    EP_HOST_ASSERT(rows + alignment <= INT32_MAX - 1024);      // (rounded up to tiles too)
     if (present(psum)) {
         EP_HOST_ASSERT(psum.ndim == 1 and psum.dtype == EP_DTYPE_I32 and contiguous(psum));
         EP_HOST_ASSERT(psum.size[0] == num_experts);
@@ -168,7 +168,7 @@ void ep_load_expert_kernels(const char* dir) {
     get(g_k.sum_weights[0], "ep_sum_weights_bf16");
     get(g_k.sum_weights[1], "ep_sum_weights_f32");
     get(g_k.sum_splits_lora, "ep_sum_splits_lora");
-    for (int i = 0; i < 3; ++i) get(g_k.lora_down[i], format("ep_lora_down_16_%d", 16 << i).c_str());
+    for (int i = 0; i < 3; ++i) get(g_k.lora_down[i], format("ep_lora_down_%d", 16 << i).c_str());
     get(g_k.lora_down_rows, "ep_lora_down_rows");
     get(g_k.expand_fill, "ep_expand_fill");
     get(g_k.expand_rows, "ep_expand_token_index_rows");

@@ -20,7 +20,6 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -232,20 +231,20 @@ struct TileFetch {
     __device__ __forceinline__ void fetch(i32x4 buffer, int i, unsigned to, int wave) const { fetch16(to + piece(i, wave) * 1024, from[i], buffer); }
 };
 
-// What a lane gives a matrix instruction over MT rows (or columns) of an operand, 16 bytes at a time: of row lane % MT, chunk
+constexpr int MT = 16;         // rows and columns of a matrix instruction
+// What a lane gives one over MT rows (or columns) of an operand, 16 bytes at a time: of row lane % MT, chunk
 // q * (64 / MT) + lane / MT of the step's eight.
-template <int MT>
 __device__ __forceinline__ u32x4 direct_fragment(const char* tile, int first, int q) {
     const int lane = lane_id(), r = lane % MT;
     return *(const u32x4*)(tile + (first + r) * 128 + (((q * (WAVE / MT) + lane / MT) ^ ((r >> 1) & 7)) << 4));
 }
 // The same of a transposed tile, columns from `first` on: two transposing reads, each of which hands the lanes of a group of 16 the columns
 // of the four 32-byte row pieces that the group reads.
-template <int MT, int T>
+template <int T>
 __device__ __forceinline__ u32x4 transposed_fragment(const char* tile, int first, int q) {
     const int lane = lane_id(), j = (lane >> 2) & 3;
-    const int row = (q * (WAVE / MT) + lane / MT) * 8 + j, column = first + (lane % MT & 16);
-    const int granule = (column >> 4) ^ (j | ((lane / MT) & 1) << 2);
+    const int row = (q * (WAVE / MT) + lane / MT) * 8 + j;
+    const int granule = (first >> 4) ^ (j | ((lane / MT) & 1) << 2);
     const lds_byte* at = (const lds_byte*)(tile + row * (T * 2) + granule * 32 + (lane & 3) * 8);
     typedef __attribute__((address_space(3))) i16x4* quad;
     union {
@@ -257,28 +256,15 @@ __device__ __forceinline__ u32x4 transposed_fragment(const char* tile, int first
     return f.v;
 }
 
-template <bool TRANSPOSED, int MT, int T>
+template <bool TRANSPOSED, int T>
 __device__ __forceinline__ u32x4 fragment(const char* tile, int first, int q) {
-    if (TRANSPOSED) return transposed_fragment<MT, T>(tile, first, q);
-    return direct_fragment<MT>(tile, first, q);
+    if (TRANSPOSED) return transposed_fragment<T>(tile, first, q);
+    return direct_fragment(tile, first, q);
 }
 
-template <int MT>
-struct Sums;
-template <>
-struct Sums<16> {
-    typedef f32x4 type;
-};
-template <>
-struct Sums<32> {
-    typedef f32x16 type;
-};
-// MT x MT sums += BF16 columns x BF16 rows
+// MT x MT sums, four a lane, += BF16 columns x BF16 rows
 __device__ __forceinline__ f32x4 multiply_add(u32x4 c, u32x4 r, f32x4 sums) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, r), sums, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 multiply_add(u32x4 c, u32x4 r, f32x16 sums) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, r), sums, 0, 0, 0);
 }
 // ... e4m3: two chunks of each
 union Chunks {
@@ -287,9 +273,6 @@ union Chunks {
 };
 __device__ __forceinline__ f32x4 multiply_add_fp8(const Chunks& c, const Chunks& r, f32x4 sums) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(c.v, r.v, sums, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 multiply_add_fp8(const Chunks& c, const Chunks& r, f32x16 sums) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(c.v, r.v, sums, 0, 0, 0, 0, 0, 0);
 }
 
 // The compiler keeps what is in front of this in front.
@@ -334,7 +317,7 @@ __device__ __forceinline__ void low_ranks(const EpGemmArgs& a, int64_t row, int 
 //
 // One workgroup computes TM x TN of the output, WR x WC waves a part each, in 32 bits.  The matrix instruction's first operand is
 // the output's columns, its second the rows: a lane then holds four neighbouring columns of one row.
-template <int TM, int TN, int WR, int WC, int MT, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false,
+template <int TM, int TN, int WR, int WC, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false,
           bool LOW_RANK = false>
 struct Gemm {
     static constexpr int WAVES = WR * WC, FM = TM / WR, FN = TN / WC, NR = FM / MT, NC = FN / MT;
@@ -367,12 +350,11 @@ struct Gemm {
         const unsigned lds0 = (unsigned)(size_t)(lds_byte*)lds;
         const int steps = valid > 0 ? ceil_div(depth, STEP) : 0;
 
-        typedef typename Sums<MT>::type sums_t;
-        sums_t acc[NR][NC];
+        f32x4 acc[NR][NC];
 #pragma unroll
         for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int j = 0; j < NC; ++j) acc[i][j] = sums_t{};
+            for (int j = 0; j < NC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
         ColumnsFetch cf;
         RowsFetch rf;
@@ -453,8 +435,8 @@ struct Gemm {
         constexpr int READ_SPAN = (PRODUCTS * 5 + 7) / 8;
         auto read_one = [&](u32x4 (&c)[HQ][NC], u32x4 (&r)[HQ][NR], int slot_rows, int slot_columns, int half, int i) {
             const int q = i / (NC + NR), k = i - q * (NC + NR);
-            if (k < NC) c[q][k] = fragment<COLUMNS_T, MT, TN>(lds + slot_columns * COLUMNS_BYTES, first_column + k * MT, half * HQ + q);
-            else r[q][k - NC] = fragment<ROWS_T, MT, TM>(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + (k - NC) * MT, half * HQ + q);
+            if (k < NC) c[q][k] = fragment<COLUMNS_T, TN>(lds + slot_columns * COLUMNS_BYTES, first_column + k * MT, half * HQ + q);
+            else r[q][k - NC] = fragment<ROWS_T, TM>(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + (k - NC) * MT, half * HQ + q);
         };
         auto multiply_one = [&](const u32x4 (&c)[HQ][NC], const u32x4 (&r)[HQ][NR], int at) {
             const int q = at / (NR * NC), i = at / NC % NR, j = at % NC;
@@ -541,22 +523,22 @@ struct Gemm {
             const float* const of_block = &table[first_column / 128 * TABLE];
             auto read_columns = [&](Chunks (&c)[HQ], int slot_columns, int j) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) c[q / 2].half[q % 2] = direct_fragment<MT>(lds + slot_columns * COLUMNS_BYTES, first_column + j * MT, q);
+                for (int q = 0; q < Q; ++q) c[q / 2].half[q % 2] = direct_fragment(lds + slot_columns * COLUMNS_BYTES, first_column + j * MT, q);
             };
             auto read_row = [&](Chunks (&r)[HQ], float& scale, int slot_rows, int i) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) r[q / 2].half[q % 2] = direct_fragment<MT>(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + i * MT, q);
+                for (int q = 0; q < Q; ++q) r[q / 2].half[q % 2] = direct_fragment(lds + ROWS_AT + slot_rows * ROWS_BYTES, first_row + i * MT, q);
                 scale = ((const float*)(lds + SF_AT + slot_rows * SF_BYTES))[first_row + i * MT + lane % MT];
             };
             auto multiply = [&](const Chunks (&c)[HQ], const Chunks (&r)[HQ]) {
-                sums_t sum = {};
+                f32x4 sum = {};
 #pragma unroll
                 for (int q = 0; q < HQ; ++q) sum = multiply_add_fp8(c[q], r[q], sum);
                 return sum;
             };
-            auto add_scaled = [&](sums_t& to, const sums_t& sum, float scale) {
+            auto add_scaled = [&](f32x4& to, const f32x4& sum, float scale) {
 #pragma unroll
-                for (int k = 0; k < MT * MT / WAVE; ++k) to[k] = __builtin_fmaf(sum[k], scale, to[k]);
+                for (int k = 0; k < 4; ++k) to[k] = __builtin_fmaf(sum[k], scale, to[k]);
             };
             if constexpr (NR >= 4) {
                 // Rows of fragments are read two ahead; behind the last of them the waves meet, and while the last two rows are multiplied the
@@ -590,7 +572,7 @@ struct Gemm {
                 }
                 for (int s = 0; s < steps; ++s) {
                     const float of_columns = of_block[s];
-                    sums_t sums[DEPTH];
+                    f32x4 sums[DEPTH];
                     // product p: of row i and column j; the last two rows column by column, so that the columns' fragments are free one by one
                     auto row_of = [](int p) { return p < LAST ? p / NC : NR - 2 + (p - LAST) % 2; };
                     auto column_of = [](int p) { return p < LAST ? p % NC : (p - LAST) / 2; };
@@ -674,14 +656,10 @@ struct Gemm {
         for (int i = 0; i < NR; ++i) {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-#pragma unroll
-                for (int g = 0; g < MT * MT / WAVE / 4; ++g) {
-                    // four neighbouring columns of row lane % MT
-                    const f32x4 v = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                    char* const to = mine + lane % MT * OUT_ROW + (j * MT + g * (WAVE / MT * 4) + lane / MT * 4) * OUT_ELEM;
-                    if (OUT32) *(f32x4*)to = v;
-                    else *(bf16x4*)to = __builtin_convertvector(v, bf16x4);
-                }
+                // four neighbouring columns of row lane % MT
+                char* const to = mine + lane % MT * OUT_ROW + (j * MT + lane / MT * 4) * OUT_ELEM;
+                if (OUT32) *(f32x4*)to = acc[i][j];
+                else *(bf16x4*)to = __builtin_convertvector(acc[i][j], bf16x4);
             }
             asm volatile("" ::: "memory");
 #pragma unroll
@@ -762,7 +740,7 @@ struct Gemm {
     }
     // Many adapters: behind the product, lane by lane with the row's own adapter, eight ranks at a time and four columns of a sum together.  The
     // time goes by the ranks and not by the number of adapters (64 rows of 27 adapters beside 128 columns: a step each was 70 us).
-    __device__ __forceinline__ static void add_adapters_by_row(const EpGemmArgs& a, typename Sums<MT>::type (&acc)[NR][NC], const char* up, int64_t first,
+    __device__ __forceinline__ static void add_adapters_by_row(const EpGemmArgs& a, f32x4 (&acc)[NR][NC], const char* up, int64_t first,
                                                                int valid, int first_row, int first_column, int num_columns) {
         const EpLoraArgs& l = a.lora;
         const int lane = lane_id();
@@ -777,8 +755,8 @@ struct Gemm {
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
 #pragma unroll
-                    for (int g = 0; g < MT * MT / WAVE; ++g) {
-                        const int column = first_column + j * MT + g / 4 * (WAVE / MT * 4) + lane / MT * 4 + g % 4;
+                    for (int g = 0; g < 4; ++g) {
+                        const int column = first_column + j * MT + lane / MT * 4 + g;
                         if (column >= num_columns) continue;
                         const bf16x8 w = *(const bf16x8*)(mine + column * l.up_ld + rank * 2);
                         float sum = acc[i][j][g];
@@ -858,56 +836,56 @@ struct Gemm {
     }
 };
 
-#define EP_GEMM_ROWS(NAME, TM, TN, WR, WC, MT, SR, SC, FP8, COLUMNS_T, GROUP)                                         \
+#define EP_GEMM_ROWS(NAME, TM, TN, WR, WC, SR, SC, FP8, COLUMNS_T, GROUP)                                         \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, MT, SR, SC, FP8, COLUMNS_T, false, false>::rows_kernel<false>(a, GROUP);                 \
+        Gemm<TM, TN, WR, WC, SR, SC, FP8, COLUMNS_T, false, false>::rows_kernel<false>(a, GROUP);                 \
     }
-typedef Gemm<64, 128, 2, 2, 16, 3, 3, false, false, false, true> SplitBf16;
-typedef Gemm<64, 128, 2, 2, 16, 3, 3, true, false, false, true> SplitFp8;
+typedef Gemm<64, 128, 2, 2, 3, 3, false, false, false, true> SplitBf16;
+typedef Gemm<64, 128, 2, 2, 3, 3, true, false, false, true> SplitFp8;
 extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_bf16(EpGemmArgs a) { SplitBf16::rows_kernel<true>(a, 1); }
 extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_fp8(EpGemmArgs a) { SplitFp8::rows_kernel<true>(a, 1); }
-#define EP_GEMM_LORA(NAME, TM, TN, WR, WC, MT, SR, SC, GROUP)                                                         \
+#define EP_GEMM_LORA(NAME, TM, TN, WR, WC, SR, SC, GROUP)                                                         \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, MT, SR, SC, false, false, false, false, true>::rows_kernel<false>(a, GROUP);             \
+        Gemm<TM, TN, WR, WC, SR, SC, false, false, false, false, true>::rows_kernel<false>(a, GROUP);             \
     }
-#define EP_GEMM_WEIGHTS(NAME, TM, TN, WR, WC, MT, SR, SC, OUT32, SPLIT, GROUP)                                        \
+#define EP_GEMM_WEIGHTS(NAME, TM, TN, WR, WC, SR, SC, OUT32, SPLIT, GROUP)                                        \
     extern "C" __global__ __launch_bounds__(WR* WC* WAVE) void NAME(EpGemmArgs a) {                                   \
-        Gemm<TM, TN, WR, WC, MT, SR, SC, false, true, true, OUT32>::weights_kernel<SPLIT>(a, GROUP);                         \
+        Gemm<TM, TN, WR, WC, SR, SC, false, true, true, OUT32>::weights_kernel<SPLIT>(a, GROUP);                         \
     }
-EP_GEMM_ROWS(ep_grouped_bf16_32x64, 32, 64, 1, 4, 16, 4, 4, false, false, 4)
-EP_GEMM_ROWS(ep_grouped_bf16_64x128, 64, 128, 2, 2, 16, 3, 3, false, false, 1)
-EP_GEMM_ROWS(ep_grouped_bf16_64x256, 64, 256, 1, 8, 16, 3, 3, false, false, 1)
-EP_GEMM_ROWS(ep_grouped_bf16_128x256, 128, 256, 2, 4, 16, 3, 3, false, false, 1)
-EP_GEMM_ROWS(ep_grouped_bf16_256x256, 256, 256, 4, 2, 16, 2, 3, false, false, 8)
-EP_GEMM_ROWS(ep_grouped_fp8_32x64, 32, 64, 1, 4, 16, 4, 4, true, false, 4)
-EP_GEMM_ROWS(ep_grouped_fp8_64x128, 64, 128, 2, 2, 16, 3, 3, true, false, 1)
-EP_GEMM_ROWS(ep_grouped_fp8_64x256, 64, 256, 1, 8, 16, 3, 3, true, false, 1)
-EP_GEMM_ROWS(ep_grouped_fp8_128x256, 128, 256, 2, 4, 16, 3, 3, true, false, 1)
-EP_GEMM_ROWS(ep_grouped_fp8_256x256, 256, 256, 2, 4, 16, 2, 2, true, false, 8)
-EP_GEMM_ROWS(ep_grouped_transposed_64x128, 64, 128, 2, 2, 16, 3, 3, false, true, 1)
-EP_GEMM_ROWS(ep_grouped_transposed_64x256, 64, 256, 1, 8, 16, 3, 3, false, true, 1)
-EP_GEMM_ROWS(ep_grouped_transposed_128x256, 128, 256, 2, 4, 16, 3, 3, false, true, 1)
-EP_GEMM_ROWS(ep_grouped_transposed_256x256, 256, 256, 2, 4, 16, 2, 3, false, true, 8)
-EP_GEMM_LORA(ep_grouped_lora_32x64, 32, 64, 1, 4, 16, 4, 4, 4)
-EP_GEMM_LORA(ep_grouped_lora_64x128, 64, 128, 2, 2, 16, 3, 3, 1)
-EP_GEMM_LORA(ep_grouped_lora_64x256, 64, 256, 1, 8, 16, 3, 3, 1)
-EP_GEMM_LORA(ep_grouped_lora_128x256, 128, 256, 2, 4, 16, 3, 3, 1)
-EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 16, 2, 3, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 16, 2, 2, false, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 16, 2, 3, false, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 16, 2, 2, true, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 16, 2, 3, true, false, 8)
-EP_GEMM_WEIGHTS(ep_grouped_split_weights, 128, 128, 2, 4, 16, 2, 2, true, true, 8)
+EP_GEMM_ROWS(ep_grouped_bf16_32x64, 32, 64, 1, 4, 4, 4, false, false, 4)
+EP_GEMM_ROWS(ep_grouped_bf16_64x128, 64, 128, 2, 2, 3, 3, false, false, 1)
+EP_GEMM_ROWS(ep_grouped_bf16_64x256, 64, 256, 1, 8, 3, 3, false, false, 1)
+EP_GEMM_ROWS(ep_grouped_bf16_128x256, 128, 256, 2, 4, 3, 3, false, false, 1)
+EP_GEMM_ROWS(ep_grouped_bf16_256x256, 256, 256, 4, 2, 2, 3, false, false, 8)
+EP_GEMM_ROWS(ep_grouped_fp8_32x64, 32, 64, 1, 4, 4, 4, true, false, 4)
+EP_GEMM_ROWS(ep_grouped_fp8_64x128, 64, 128, 2, 2, 3, 3, true, false, 1)
+EP_GEMM_ROWS(ep_grouped_fp8_64x256, 64, 256, 1, 8, 3, 3, true, false, 1)
+EP_GEMM_ROWS(ep_grouped_fp8_128x256, 128, 256, 2, 4, 3, 3, true, false, 1)
+EP_GEMM_ROWS(ep_grouped_fp8_256x256, 256, 256, 2, 4, 2, 2, true, false, 8)
+EP_GEMM_ROWS(ep_grouped_transposed_64x128, 64, 128, 2, 2, 3, 3, false, true, 1)
+EP_GEMM_ROWS(ep_grouped_transposed_64x256, 64, 256, 1, 8, 3, 3, false, true, 1)
+EP_GEMM_ROWS(ep_grouped_transposed_128x256, 128, 256, 2, 4, 3, 3, false, true, 1)
+EP_GEMM_ROWS(ep_grouped_transposed_256x256, 256, 256, 2, 4, 2, 3, false, true, 8)
+EP_GEMM_LORA(ep_grouped_lora_32x64, 32, 64, 1, 4, 4, 4, 4)
+EP_GEMM_LORA(ep_grouped_lora_64x128, 64, 128, 2, 2, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_64x256, 64, 256, 1, 8, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_128x256, 128, 256, 2, 4, 3, 3, 1)
+EP_GEMM_LORA(ep_grouped_lora_256x256, 256, 256, 4, 2, 2, 3, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_128x128, 128, 128, 2, 4, 2, 2, false, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_bf16_256x256, 256, 256, 2, 4, 2, 3, false, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_128x128, 128, 128, 2, 4, 2, 2, true, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_weights_f32_256x256, 256, 256, 2, 4, 2, 3, true, false, 8)
+EP_GEMM_WEIGHTS(ep_grouped_split_weights, 128, 128, 2, 4, 2, 2, true, true, 8)
 
 // ---- low-rank adapters: rows times the first matrix ---------------------------------------------------------
 //
-// low[chunk][r] = scale[a] * sum over the chunk's channels of down[a][e] rows[r].  A workgroup has ROWS rows of an expert, a chunk of the
+// low[chunk][r] = scale[a] * sum over the chunk's channels of down[a][e] rows[r].  A workgroup has 16 rows of an expert, a chunk of the
 // depth, which its four waves share 64 or 128 channels at a time, and every `slots`-th of the adapters that its rows have: all rows are
 // multiplied with an adapter's matrix, and the rows that have it keep what they get.  Operands go from memory straight to
 // registers: nothing is used twice but by the neighbouring waves, out of the caches.
-template <int ROWS, int RANKS>
+template <int RANKS>
 __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a, int block) {
-    constexpr int NR = ROWS / 16, NK = RANKS / 16, PARTS = RANKS > 32 ? 2 : 4;
+    constexpr int ROWS = 16, NK = RANKS / 16, PARTS = RANKS > 32 ? 2 : 4;
     __shared__ __attribute__((aligned(16))) float sums[4][ROWS][RANKS + 4];
     const EpLoraArgs& l = a.lora;
     const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
@@ -929,30 +907,25 @@ __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a, int block) {
         if (n++ % l.slots != slot) continue;
         const int number = __builtin_amdgcn_readlane(of_row, __builtin_ctzll(leaders));
         const buffer_t w_buffer = bounded(l.down + number * l.down_adapter + t.expert * l.down_expert, (unsigned)((l.rank - 1) * l.down_ld) + a.depth * 2);
-        f32x4 acc[NR][NK];
+        f32x4 acc[NK];
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int j = 0; j < NK; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NK; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
         // (a turn's operands are on their way while the one before is multiplied)
-        u32x4 x[2][PARTS][NR], w[2][PARTS][NK];
-        auto load = [&](int k0, u32x4 (&x)[PARTS][NR], u32x4 (&w)[PARTS][NK]) {
+        u32x4 x[2][PARTS], w[2][PARTS][NK];
+        auto load = [&](int k0, u32x4 (&x)[PARTS], u32x4 (&w)[PARTS][NK]) {
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 const int k = k0 + p * 32 + (lane >> 4) * 8;
-#pragma unroll
-                for (int i = 0; i < NR; ++i) x[p][i] = load16(x_buffer, k < end ? (unsigned)((i * 16 + (lane & 15)) * a.rows_ld) + k * 2 : OUTSIDE);
+                x[p] = load16(x_buffer, k < end ? (unsigned)((lane & 15) * a.rows_ld) + k * 2 : OUTSIDE);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) w[p][j] = load16(w_buffer, k < end ? (unsigned)((j * 16 + (lane & 15)) * l.down_ld) + k * 2 : OUTSIDE);
             }
         };
-        auto multiply = [&](const u32x4 (&x)[PARTS][NR], const u32x4 (&w)[PARTS][NK]) {
+        auto multiply = [&](const u32x4 (&x)[PARTS], const u32x4 (&w)[PARTS][NK]) {
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int i = 0; i < NR; ++i)
-#pragma unroll
-                    for (int j = 0; j < NK; ++j) acc[i][j] = multiply_add(w[p][j], x[p][i], acc[i][j]);
+                for (int j = 0; j < NK; ++j) acc[j] = multiply_add(w[p][j], x[p], acc[j]);
         };
         constexpr int TURN = 128 * PARTS;
         const int k0 = begin + wave * 32 * PARTS;
@@ -964,9 +937,7 @@ __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a, int block) {
             multiply(x[1], w[1]);
         }
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int j = 0; j < NK; ++j) *(f32x4*)&sums[wave][i * 16 + (lane & 15)][j * 16 + (lane >> 4) * 4] = acc[i][j];
+        for (int j = 0; j < NK; ++j) *(f32x4*)&sums[wave][lane & 15][j * 16 + (lane >> 4) * 4] = acc[j];
         __syncthreads();
         const float scale = l.scales != nullptr ? l.scales[number] : 1.0f;
         for (int i = threadIdx.x; i < ROWS * (RANKS / 4); i += 256) {
@@ -978,14 +949,14 @@ __device__ __forceinline__ void lora_down_body(const EpGemmArgs& a, int block) {
         __syncthreads();
     }
 }
-#define EP_LORA_DOWN(ROWS, RANKS) \
-    extern "C" __global__ __launch_bounds__(256) void ep_lora_down_##ROWS##_##RANKS(EpGemmArgs a) { lora_down_body<ROWS, RANKS>(a, blockIdx.x); }
-EP_LORA_DOWN(16, 16)
-EP_LORA_DOWN(16, 32)
-EP_LORA_DOWN(16, 64)
+#define EP_LORA_DOWN(RANKS) \
+    extern "C" __global__ __launch_bounds__(256) void ep_lora_down_##RANKS(EpGemmArgs a) { lora_down_body<RANKS>(a, blockIdx.x); }
+EP_LORA_DOWN(16)
+EP_LORA_DOWN(32)
+EP_LORA_DOWN(64)
 
 // Many rows: the same sums as a product of 64 rows with the matrices of as many adapters as have 64 ranks together.
-typedef Gemm<64, 64, 4, 1, 16, 3, 3, false, false, false, true, false, true> LowRank;
+typedef Gemm<64, 64, 4, 1, 3, 3, false, false, false, true, false, true> LowRank;
 extern "C" __global__ __launch_bounds__(256) void ep_lora_down_rows(EpGemmArgs a) {
     const EpLoraArgs& l = a.lora;
     const int chunk = blockIdx.x % l.chunks;
@@ -1016,7 +987,7 @@ extern "C" __global__ __launch_bounds__(256) void ep_lora_down_rows(EpGemmArgs a
     extern "C" __global__ __launch_bounds__(256) void ep_grouped_split_lora_##RANKS(EpGemmArgs a) {                   \
         const int behind = (int)blockIdx.x - ((int)gridDim.x - a.lora.blocks);                                        \
         if (behind < 0) SplitBf16::rows_kernel<true>(a, 1, blockIdx.x);                                               \
-        else lora_down_body<16, RANKS>(a, behind);                                                                    \
+        else lora_down_body<RANKS>(a, behind);                                                                    \
     }
 EP_LORA_SPLIT(16)
 EP_LORA_SPLIT(32)

@@ -5,9 +5,11 @@
 // contract and every launch lives behind the C ABI in libdeep_ep_hip.so.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <memory>
@@ -597,6 +599,15 @@ void on_current_device(std::initializer_list<const at::Tensor*> tensors) {
 const at::Tensor* of(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 
 // (the result, allocated where the caller brings none)
+// A result where an operand lies would be read again by other workgroups.
+void apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> operands) {
+    for (const at::Tensor* t : operands) {
+        if (t == nullptr) continue;
+        const auto overlap = at::get_overlap_status(out, *t);
+        EP_PY_ASSERT(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial);
+    }
+}
+
 at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf,
                        const OptTensor& psum, int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
     on_current_device({&x, of(x_sf), &weight, of(weight_sf), of(psum), of(out)});
@@ -609,6 +620,7 @@ at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const O
         a.weight_sf = expert_matrix(*weight_sf, a.weight_sf_expert_stride);
     }
     a.psum_num_recv_tokens_per_expert = desc(psum);
+    if (out.has_value()) apart(*out, {&x, of(x_sf), &weight, of(weight_sf), of(psum)});
     const at::Tensor y = out.has_value() ? *out : alloc({x.size(0), weight.size(transpose_weight ? -1 : -2)}, at::kBFloat16, x.device());
     a.out = desc(y);
     a.num_experts = num_matrices(weight);
@@ -658,6 +670,7 @@ at::Tensor grouped_lora_linear(const at::Tensor& x, const at::Tensor& weight, co
                                const at::Tensor& adapter_idx, const OptTensor& scales, const OptTensor& psum, int alignment, const OptTensor& out,
                                int zero_rows) {
     on_current_device({&lora_a, &lora_b, &adapter_idx, of(scales)});
+    if (out.has_value()) apart(*out, {&lora_a, &lora_b, &adapter_idx, of(scales)});
     ep_grouped_lora_args_t a{};
     const at::Tensor y = fill_linear(a.linear, x, std::nullopt, weight, std::nullopt, psum, alignment, out, zero_rows, false);
     EP_PY_ASSERT(lora_a.dim() >= 3);
@@ -690,6 +703,7 @@ at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, cons
                                const OptTensor& out, bool accumulate) {
     on_current_device({&grad, &x, of(psum), of(out)});
     EP_PY_ASSERT(grad.dim() == 2 && x.dim() == 2);
+    if (out.has_value()) apart(*out, {&grad, &x, of(psum)});
     const at::Tensor w = out.has_value() ? *out : alloc({num_experts, grad.size(1), x.size(1)}, at::kBFloat16, x.device());
     ep_grouped_weight_grad_args_t a{};
     a.grad = desc(grad);
@@ -715,6 +729,8 @@ std::tuple<at::Tensor, OptTensor> swiglu(const at::Tensor& h, const OptTensor& w
                                          bool quantise, const OptTensor& out, const OptTensor& out_sf, int zero_rows) {
     on_current_device({&h, of(weights), of(psum), of(out), of(out_sf)});
     EP_PY_ASSERT(h.dim() == 2);
+    if (out.has_value()) apart(*out, {&h, of(weights), of(psum)});
+    if (out_sf.has_value()) apart(*out_sf, {&h, of(weights), of(psum), of(out)});
     const int64_t rows = h.size(0), channels = h.size(1) / 2;
     const at::Tensor y = out.has_value() ? *out : alloc({rows, channels}, quantise ? at::kFloat8_e4m3fn : at::kBFloat16, h.device());
     OptTensor sf = out_sf;
@@ -774,6 +790,22 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
     return (*error)(std::move(grads));
 }
 
+// A captured pass whose leaves an eager graph, still alive, has tied to another stream would bring that stream into the capture, which
+// breaks the capture and, with it, the process: an error in time.
+void in_one_stream_if_captured() {
+    const auto current = c10::hip::getCurrentHIPStream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::get_current_node();
+    for (const auto& edge : node->next_edges()) {
+        if (!edge.is_valid() || dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
+        const auto stream = edge.function->stream();
+        if (stream.has_value() && stream->id() != current.id())
+            throw std::runtime_error("a backward pass is captured into a graph while an eager one of the same leaves lives: end that one first, or capture "
+                                     "grouped_linear_grad and swiglu_grad");
+    }
+}
+
 struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& psum, int64_t alignment,
                               int64_t zero_rows) {
@@ -787,6 +819,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
         const int alignment = (int)ctx->saved_data["alignment"].toInt();
         torch::autograd::variable_list out(5);
         if (!grads[0].defined()) return out;
+        in_one_stream_if_captured();
         {
             at::NoGradGuard no_grad;
             const at::Tensor grad = rows_of(grads[0]);
@@ -812,6 +845,7 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
         const auto saved = ctx->get_saved_variables();
         torch::autograd::variable_list out(6);
         if (!grads[0].defined()) return out;
+        in_one_stream_if_captured();
         {
             at::NoGradGuard no_grad;
             auto [of_h, of_weights] = swiglu_grad(rows_of(grads[0]), saved[0], present(saved[1]), present(saved[2]), (int)ctx->saved_data["num_experts"].toInt(),

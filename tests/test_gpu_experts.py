@@ -581,6 +581,70 @@ def test_captured_with_a_dispatch_and_replayed():
         torch.cuda.synchronize()
 
 
+def test_results_do_not_lie_on_operands():
+    x, w, psum = _dev(U.normal(1, 8, 64)), _dev(U.normal(2, 64, 64)), _dev(torch.tensor([8], dtype=torch.int32))
+    a, b, idx = _dev(U.normal(3, 1, 8, 64)), _dev(U.normal(4, 1, 64, 8)), torch.zeros(8, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError):
+        deep_ep.grouped_linear(x, w, out=x)
+    with pytest.raises(RuntimeError):
+        deep_ep.grouped_linear(x, w, out=w[8:16])
+    with pytest.raises(RuntimeError):
+        deep_ep.grouped_lora_linear(x, w, a, b, idx, out=x)
+    with pytest.raises(RuntimeError):
+        deep_ep.grouped_linear_grad(w, w, w, need_x=False, grad_weight=w)
+    h = _dev(U.normal(5, 64, 64))
+    with pytest.raises(RuntimeError):
+        deep_ep.swiglu(h, out=h.view(-1)[:64 * 32].view(64, 32))
+
+
+def test_captured_backward_pass_and_replayed():
+    layout = U.Layout([300, 20], 16)
+    psum = layout.on(DEV)
+    inputs = [_dev(U.normal(1, layout.rows, 256)), _dev(U.normal(2, 2, 256, 256)), torch.rand(layout.rows, device=DEV), _dev(U.normal(3, layout.rows, 128))]
+
+    def step(x, w, g, grad):
+        x, w, g = (t.detach().requires_grad_() for t in (x, w, g))
+        deep_ep.swiglu(deep_ep.grouped_linear(x, w, psum), psum, g, do_zero_padding=True).backward(grad)
+        return x.grad, w.grad, g.grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*inputs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*inputs)
+    for seed in range(4):
+        inputs[0].copy_(U.normal(10 + seed, layout.rows, 256))
+        inputs[3].copy_(U.normal(20 + seed, layout.rows, 128))
+        graph.replay()
+        got = [t.clone() for t in captured]
+        for g, w in zip(got, step(*inputs)):
+            assert torch.equal(g, w)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('kind', ['linear', 'swiglu'])
+def test_captured_backward_pass_beside_an_eager_graph_is_refused(kind):
+    x, w = _dev(U.normal(1, 8, 64)).requires_grad_(), _dev(U.normal(2, 64, 64)).requires_grad_()
+    run = (lambda: deep_ep.grouped_linear(x, w)) if kind == 'linear' else (lambda: deep_ep.swiglu(x))
+    eager = run()
+    grad = torch.ones_like(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run()
+        with pytest.raises(RuntimeError, match='while an eager one of the same leaves lives'):
+            y.backward(grad)
+    graph.replay()
+    assert x.grad is None and torch.equal(y.detach(), eager.detach())
+    eager.backward(grad)
+    if kind == 'linear':
+        assert torch.equal(w.grad, deep_ep.grouped_linear_grad(grad, x.detach(), w.detach())[1])
+    else:
+        assert torch.equal(x.grad, deep_ep.swiglu_grad(grad, x.detach())[0])
+
+
 def test_on_another_stream():
     layout = U.Layout([300, 20], 16)
     x, w = _dev(U.normal(1, layout.rows, 256)), _dev(U.normal(2, 2, 256, 256))

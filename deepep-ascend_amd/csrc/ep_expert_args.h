@@ -41,7 +41,6 @@ struct EpGemmArgs {
     int num_out_rows;             // weight gradient: rows of the output of one expert
     int column_tiles, row_tiles;  // (row_tiles: weight gradient)
     int accumulate;               // weight gradient in 32 bits: added to what is there
-    int few_rows;                 // weight gradient: experts have few rows on average
     int splits, split_depth;      // the depth in so many parts (of split_depth channels), sums of each in `partial`
     float* partial;               // [splits, rows, num_columns]
     EpLoraArgs lora;

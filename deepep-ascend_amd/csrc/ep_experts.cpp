@@ -191,7 +191,7 @@ struct LoraPlan {
 };
 static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
     LoraPlan p{};
-    p.rows = rows <= 2048 ? 16 : 64;
+    p.rows = rows <= 1024 ? 16 : 64;
     const int64_t tiles = std::max<int64_t>(1, row_tiles_bound(rows, num_experts, p.rows));
     p.slots = p.rows == 16 ? (int)std::clamp<int64_t>(ceil_div(512, tiles), 1, std::min<int64_t>(p.rows, std::max<int64_t>(rows, 1))) : 1;
     const int64_t steps = ceil_div(depth, EP_LORA_STEP), chunks = std::clamp<int64_t>(ceil_div(512, tiles * p.slots), 1, std::min<int64_t>(steps, 16));
@@ -409,11 +409,10 @@ int ep_grouped_weight_grad(const ep_grouped_weight_grad_args_t* args) {
         g.splits = p.splits;
         g.partial = p.splits > 1 ? (float*)args->workspace : nullptr;
         g.accumulate = args->accumulate != 0;
-        g.few_rows = mean_rows(g.layout.num_rows, g.layout.num_experts, g.layout.alignment) <= 256;
-        const int64_t tiles = (int64_t)experts * g.row_tiles * p.splits;
-        EP_HOST_ASSERT(tiles <= INT32_MAX / (8 * (int64_t)g.column_tiles));
+        EP_HOST_ASSERT((int64_t)g.row_tiles * p.splits <= INT32_MAX / (16 * (int64_t)g.column_tiles));
+        const int64_t blocks = experts * align_up((int64_t)g.row_tiles * g.column_tiles * p.splits, 8);
         const ExpertKernels& k = kernels();
-        launch(p.splits > 1 ? k.split_weights : k.weights[f32 ? 1 : 0][p.large ? 1 : 0], align_up(tiles * g.column_tiles, 8), 512, args->stream, g);
+        launch(p.splits > 1 ? k.split_weights : k.weights[f32 ? 1 : 0][p.large ? 1 : 0], blocks, 512, args->stream, g);
         if (p.splits > 1) launch(k.sum_weights[f32 ? 1 : 0], ceil_div((int64_t)experts * g.num_out_rows * g.num_columns, 1024), 256, args->stream, g);
     });
 }

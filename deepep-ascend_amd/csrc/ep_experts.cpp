@@ -98,7 +98,7 @@ struct Plan {
 //   64 experts, 2560 to 1536, 7147 rows 162 160 124 121, of Zipf(0.6) popularity 161 163 146 131
 //   32 experts, 4096 to 4096, 3500 rows 309 240 199 281, 6000 rows 521 456 257 311
 // (the last two are bound by the weights).  Experts end inside a tile, half of one on average.
-Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool transposed) {
+Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int64_t columns, bool transposed, bool adapters) {
     const int64_t mean = mean_rows(rows, num_experts, alignment);
     const int64_t cost[kNumTiles] = {0, 55, 48, 62, 100}, slots[kNumTiles] = {512, 512, 256, 256, 256};
     int64_t tiles[kNumTiles], best = INT64_MAX;
@@ -117,10 +117,18 @@ Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int6
     // 122 -> 108 us)
     if (p.tile == kTile64Wide and tiles[kTile64Wide] <= 256) p.tile = kTile64;
     if (transposed) return p;
+    // Less than a round of 64 x 128 tiles: smaller ones, or the depth in parts, whose sum is a launch of its own and as many times 32 bits of the
+    // result.  In us, 32 x 64 / 64 x 128 in 2, 4, 8, 16 parts:
+    //   2048 channels to 2048, 64 rows (16 tiles of 64 x 128) 10 / 12 10 11 11, 256 rows (64) 11 / 14 14 16 16
+    //   4096 to 2048, 64 rows (16) 17 / 17 13 15 14, 128 rows (32) 17 / 17 13 14 17, 256 rows (64) 18 / 18 19 20 27
+    //   7168 to 4096, 64 rows (32) 27 / 25 18 18 20, 128 rows (64) 28 / 26 25 28 34, 256 rows (128) 38 / 41 44 50 62
+    // and FP8 the same.  Beside adapters 32 x 64 tiles need a launch of their own too, for the low-rank rows, and the parts do not:
+    //   2048 to 2048, 64 rows (16) 29 / 16 14 14 14, 7168 to 4096, 64 rows (32) 53 / 31 25 25 28, 256 rows (128) 63 / 55 64 68 79
     if (tiles[kTile64] < 256) {
+        const int64_t few = tiles[kTile64], parts = std::clamp<int64_t>(128 / few, adapters ? 2 : 4, 16);
+        const bool split = adapters or (few <= 64 and depth >= std::max<int64_t>(2560, 80 * few));
         const int64_t steps = ceil_div(depth, 128);
-        p.splits = (int)std::clamp<int64_t>(512 / tiles[kTile64], 1, std::max<int64_t>(1, std::min<int64_t>(16, steps / 6)));
-        p.split_depth = (int)(ceil_div(steps, p.splits) * 128);
+        p.split_depth = (int)(ceil_div(steps, split ? std::min(parts, std::max<int64_t>(1, steps / 2)) : 1) * 128);
         p.splits = (int)ceil_div(depth, p.split_depth);
         p.tile = p.splits > 1 ? kTile64 : kTile32;
     }
@@ -128,7 +136,7 @@ Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int6
 }
 
 // The gradient of weights: tiles of 256 x 256 as soon as they fill the chip; where those of 128 x 128 do not either and rows are many, rows
-// in parts.
+// in parts of 600 at least (8192 rows, one expert's 1024 x 1024: 74 -> 34 us; 1024 of each of eight experts, 512 x 512, in two parts: 15 -> 18).
 struct WeightsPlan {
     bool large;
     int splits;
@@ -137,7 +145,7 @@ WeightsPlan plan_weights(int64_t rows, int num_experts, int alignment, int64_t o
     WeightsPlan p{num_experts * ceil_div(out_rows, 256) * ceil_div(out_columns, 256) >= 256, 1};
     const int64_t tiles = num_experts * ceil_div(out_rows, 128) * ceil_div(out_columns, 128);
     if (not p.large and tiles < 256)
-        p.splits = (int)std::clamp<int64_t>(512 / tiles, 1, std::clamp<int64_t>(mean_rows(rows, num_experts, alignment) / 512, 1, 32));
+        p.splits = (int)std::clamp<int64_t>(512 / tiles, 1, std::clamp<int64_t>(mean_rows(rows, num_experts, alignment) / 600, 1, 32));
     return p;
 }
 
@@ -185,10 +193,13 @@ void ep_load_expert_kernels(const char* dir) {
 extern "C" {
 
 // How the rows times the adapters' first matrices are split: rows of a workgroup's tile, chunks of the depth, workgroups that share the
-// adapters of a tile.
+// adapters of a tile; 512 workgroups in all, two a CU, where there are so many.
 struct LoraPlan {
     int rows, chunks, chunk_depth, slots;
 };
+// Up to 1024 rows tiles of 16 rows, adapter by adapter; more: 64 rows and as many adapters as have 64 ranks at once.  One expert, 4096 channels to
+// 4096, 16 ranks, in us, 4 / 32 adapters: 128 rows 27 / 28 (the other 32 / 59), 512 rows 65 / 73 (60 / 92), 2048 rows 86 / 162 (81 / 148),
+// 4096 rows 144 / 281 (134 / 217).
 static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
     LoraPlan p{};
     p.rows = rows <= 1024 ? 16 : 64;
@@ -250,7 +261,7 @@ static EpGemmArgs linear_args(const ep_grouped_linear_args_t* args) {
 // The launches of a product of rows; `workspace`: where the parts of a split depth go, if there is room.
 static void launch_rows(EpGemmArgs& g, int kind, const LoraPlan* lora, void* workspace, int64_t workspace_bytes, void* stream) {
     const EpExpertLayout& l = g.layout;
-    Plan p = plan_rows(l.num_rows, l.num_experts, l.alignment, g.depth, g.num_columns, kind == kKindTransposed);
+    Plan p = plan_rows(l.num_rows, l.num_experts, l.alignment, g.depth, g.num_columns, kind == kKindTransposed, kind == kKindLora);
     const ExpertKernels& k = kernels();
     if (p.splits > 1 and (int64_t)p.splits * l.num_rows * g.num_columns * 4 > workspace_bytes) p = Plan{kTile32, 1, 0};
     const Tile& t = kTiles[p.tile];
@@ -274,11 +285,11 @@ static void launch_rows(EpGemmArgs& g, int kind, const LoraPlan* lora, void* wor
     launch(lora != nullptr ? k.sum_splits_lora : k.sum_splits, ceil_div((int64_t)l.num_rows * ceil_div(g.num_columns, 512), 4), 256, stream, g);
 }
 
-int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns) {
+int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns, int adapters) {
     if (num_rows <= 0 or num_rows > INT32_MAX or num_experts <= 0 or expert_alignment <= 0 or depth <= 0 or depth > INT32_MAX / 2 or num_columns <= 0 or
         num_columns > INT32_MAX / 2)
         return 0;
-    const Plan p = plan_rows(num_rows, num_experts, expert_alignment, depth, num_columns, false);
+    const Plan p = plan_rows(num_rows, num_experts, expert_alignment, depth, num_columns, false, adapters != 0);
     return p.splits > 1 ? (int64_t)p.splits * num_rows * num_columns * 4 : 0;
 }
 

@@ -631,9 +631,9 @@ at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const O
     return y;
 }
 
-at::Tensor linear_workspace(ep_grouped_linear_args_t& a, const at::Device& device) {
+at::Tensor linear_workspace(ep_grouped_linear_args_t& a, const at::Device& device, bool adapters) {
     if (a.transpose_weight) return {};
-    a.workspace_bytes = ep_grouped_linear_workspace_bytes(a.x.size[0], a.num_experts, a.expert_alignment, a.x.size[1], a.weight.size[0]);
+    a.workspace_bytes = ep_grouped_linear_workspace_bytes(a.x.size[0], a.num_experts, a.expert_alignment, a.x.size[1], a.weight.size[0], adapters);
     if (a.workspace_bytes == 0) return {};
     const at::Tensor workspace = alloc({a.workspace_bytes}, at::kByte, device);
     a.workspace = workspace.data_ptr();
@@ -644,7 +644,7 @@ at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::
                           int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
     ep_grouped_linear_args_t a{};
     const at::Tensor y = fill_linear(a, x, x_sf, weight, weight_sf, psum, alignment, out, zero_rows, transpose_weight);
-    const at::Tensor workspace = linear_workspace(a, x.device());
+    const at::Tensor workspace = linear_workspace(a, x.device(), false);
     check(ep_grouped_linear(&a));
     return y;
 }
@@ -685,7 +685,7 @@ at::Tensor grouped_lora_linear(const at::Tensor& x, const at::Tensor& weight, co
         workspace = alloc({a.workspace_bytes}, at::kByte, x.device());
         a.workspace = workspace.data_ptr();
     }
-    const at::Tensor of_linear = linear_workspace(a.linear, x.device());
+    const at::Tensor of_linear = linear_workspace(a.linear, x.device(), true);
     check(ep_grouped_lora_linear(&a));
     return y;
 }

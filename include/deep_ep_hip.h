@@ -342,7 +342,8 @@ typedef struct ep_grouped_linear_args {
     int64_t workspace_bytes;            /* tiles is split over its depth */
     void* stream;
 } ep_grouped_linear_args_t;
-int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns);
+/* adapters: 1 for ep_grouped_lora_linear. */
+int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int expert_alignment, int64_t depth, int64_t num_columns, int adapters);
 /* out[m] = W[e(m)] x[m].  FP8: sums over groups of 128 channels, each scaled by x_sf[m,g] * weight_sf[e(m),n/128,g]. */
 int ep_grouped_linear(const ep_grouped_linear_args_t* args);
 

@@ -87,6 +87,9 @@ int64_t mean_rows(int64_t rows, int num_experts, int alignment) {
     return ceil_div(std::max<int64_t>(rows - (int64_t)(alignment - 1) * num_experts, std::min<int64_t>(rows, num_experts)), num_experts);
 }
 
+// Rows up to which the low-rank rows are made in tiles of 16 (lora_plan), in one launch with the parts of a product.
+constexpr int64_t kFewLoraRows = 1024;
+
 // How a product of rows is launched: its tile, and in how many parts of the depth.
 struct Plan {
     int tile, splits, split_depth;
@@ -125,8 +128,9 @@ Plan plan_rows(int64_t rows, int num_experts, int alignment, int64_t depth, int6
     // and FP8 the same.  Beside adapters 32 x 64 tiles need a launch of their own too, for the low-rank rows, and the parts do not:
     //   2048 to 2048, 64 rows (16) 29 / 16 14 14 14, 7168 to 4096, 64 rows (32) 53 / 31 25 25 28, 256 rows (128) 63 / 55 64 68 79
     if (tiles[kTile64] < 256) {
-        const int64_t few = tiles[kTile64], parts = std::clamp<int64_t>(128 / few, adapters ? 2 : 4, 16);
-        const bool split = adapters or (few <= 64 and depth >= std::max<int64_t>(2560, 80 * few));
+        const bool one_launch = adapters and rows <= kFewLoraRows;
+        const int64_t few = tiles[kTile64], parts = std::clamp<int64_t>(128 / few, one_launch ? 2 : 4, 16);
+        const bool split = one_launch or (few <= 64 and depth >= std::max<int64_t>(2560, 80 * few));
         const int64_t steps = ceil_div(depth, 128);
         p.split_depth = (int)(ceil_div(steps, split ? std::min(parts, std::max<int64_t>(1, steps / 2)) : 1) * 128);
         p.splits = (int)ceil_div(depth, p.split_depth);
@@ -197,12 +201,12 @@ extern "C" {
 struct LoraPlan {
     int rows, chunks, chunk_depth, slots;
 };
-// Up to 1024 rows tiles of 16 rows, adapter by adapter; more: 64 rows and as many adapters as have 64 ranks at once.  One expert, 4096 channels to
+// Up to kFewLoraRows tiles of 16 rows, adapter by adapter; more: 64 rows and as many adapters as have 64 ranks at once.  One expert, 4096 channels to
 // 4096, 16 ranks, in us, 4 / 32 adapters: 128 rows 27 / 28 (the other 32 / 59), 512 rows 65 / 73 (60 / 92), 2048 rows 86 / 162 (81 / 148),
 // 4096 rows 144 / 281 (134 / 217).
 static LoraPlan lora_plan(int64_t rows, int num_experts, int64_t depth) {
     LoraPlan p{};
-    p.rows = rows <= 1024 ? 16 : 64;
+    p.rows = rows <= kFewLoraRows ? 16 : 64;
     const int64_t tiles = std::max<int64_t>(1, row_tiles_bound(rows, num_experts, p.rows));
     p.slots = p.rows == 16 ? (int)std::clamp<int64_t>(ceil_div(512, tiles), 1, std::min<int64_t>(p.rows, std::max<int64_t>(rows, 1))) : 1;
     const int64_t steps = ceil_div(depth, EP_LORA_STEP), chunks = std::clamp<int64_t>(ceil_div(512, tiles * p.slots), 1, std::min<int64_t>(steps, 16));

@@ -388,6 +388,36 @@ def test_views_of_rows_scales_and_results():
     assert torch.equal(deep_ep.swiglu(wide_h[:, 256:768], layout.on(DEV), do_zero_padding=True)[covered], a[covered])
 
 
+def test_offsets_past_32_bits():
+    """Rows 4 MiB apart, experts 4 GiB apart: what contiguous tensors give, to the last bit."""
+    layout = U.Layout([700, 0, 400], 1)
+    rows, experts, ld, far = layout.rows, 3, 2 << 20, (2 << 30) + 64
+    big = [torch.empty(rows * ld, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    wide = torch.empty(experts * far, dtype=torch.bfloat16, device=DEV)
+
+    def put(buffer, t):
+        return buffer.as_strided(t.shape, (ld, 1)).copy_(t)
+    x, w, h = _dev(U.normal(1, rows, 256)), _dev(U.normal(2, experts, 128, 256)), _dev(U.normal(3, rows, 512))
+    vw = wide.as_strided(w.shape, (far, 256, 1)).copy_(w)
+    vx, out = put(big[0], x), big[1].as_strided((rows, 128), (ld, 1))
+    psum = layout.on(DEV)
+    want = deep_ep.grouped_linear(x, w, psum)
+    assert torch.equal(deep_ep.grouped_linear(vx, vw, psum, out=out), want)
+    gx, gw = deep_ep.grouped_linear_grad(want, x, w, psum)
+    a, b = _dev(U.normal(4, 2, experts, 16, 256)), _dev(U.normal(5, 2, experts, 128, 16))
+    idx = (torch.arange(rows, dtype=torch.int32) % 3 - 1).to(DEV)
+    lora = deep_ep.grouped_lora_linear(x, w, a, b, idx, psum)
+    assert torch.equal(deep_ep.grouped_lora_linear(vx, vw, a, b, idx, psum, out=out), lora)
+    out.copy_(want)
+    vgx, vgw = deep_ep.grouped_linear_grad(out, vx, vw, psum, grad_weight=vw)
+    assert torch.equal(vgx, gx) and torch.equal(vgw, gw)
+    one = deep_ep.grouped_linear(x[:40], w[0])
+    assert torch.equal(deep_ep.grouped_linear(vx[-40:].copy_(x[:40]), vw[2].copy_(w[0]), out=out[-40:]), one)
+    vh, out = put(big[0], h), big[1].as_strided((rows, 256), (ld, 1))
+    assert torch.equal(deep_ep.swiglu(vh, psum, out=out), deep_ep.swiglu(h, psum))
+    assert torch.equal(deep_ep.swiglu_grad(out, vh, psum)[0], deep_ep.swiglu_grad(deep_ep.swiglu(h, psum), h, psum)[0])
+
+
 def test_counts_beyond_the_tensors_stay_inside():
     """Whatever the counts say, no row outside the tensors is touched (an expert that ends behind the last row ends with it)."""
     x, w = _dev(U.normal(1, 40, 64)), _dev(U.normal(2, 3, 32, 64))

@@ -491,6 +491,16 @@ struct Gemm {
                         for (int i = 0; i < PRODUCTS; ++i) multiply_one(c, r, i);
                     }
                 });
+                // Rows of the tile without an adapter had zeros in its step.  Where it holds infinities or NaN these are no zeros any more, nor is
+                // the rest of an infinite low-rank row: such a wave's rows take their own adapters only, behind the product.
+                float probe = 0.f;
+#pragma unroll
+                for (int i = 0; i < NR * NC * 4; ++i) probe = __builtin_fmaf(acc[i / (NC * 4)][i / 4 % NC][i % 4], 0.f, probe);
+                by_row = __ballot(probe != probe) != 0;
+                if (by_row) {
+#pragma unroll
+                    for (int i = 0; i < NR * NC; ++i) acc[i / NC][i % NC] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
             }
         }
         if (steps > 0 && !(FP8 && NR >= 4)) fetch_all(begin_fetch(SR - 1, SR - 1, SC - 1, SC - 1), 0);

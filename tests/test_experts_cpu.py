@@ -244,3 +244,14 @@ def test_what_has_no_gradient_is_refused():
         deep_ep.grouped_lora_linear(x, w, w[None], w[None], torch.zeros(4, dtype=torch.int32))
     with pytest.raises(AssertionError, match='pair'):
         deep_ep.swiglu(x.detach(), out=torch.zeros(4, 8, dtype=torch.bfloat16), fused_fp8_quant=True)
+
+
+def test_code_object_is_built_with_its_kernels():
+    import deep_ep
+    path = os.path.join(os.path.dirname(deep_ep.__file__), 'lib', 'ep_experts.hsaco')
+    with open(path, 'rb') as f:
+        data = f.read()
+    assert b'gfx950' in data
+    for name in ('ep_grouped_bf16_256x256', 'ep_grouped_fp8_64x256', 'ep_grouped_transposed_128x256', 'ep_grouped_lora_32x64', 'ep_grouped_split_lora_64',
+                 'ep_grouped_weights_f32_256x256', 'ep_lora_down_rows', 'ep_sum_splits', 'ep_swiglu_fp8', 'ep_swiglu_gradients', 'ep_expand_token_index_rows'):
+        assert name.encode() in data, name

@@ -343,6 +343,46 @@ def test_lora_beside_a_shared_projection(rows):
     U.assert_sum(y, *U.linear(x, w[:1], U.Layout([rows], 1)), 1024)
 
 
+@pytest.mark.parametrize('rows,columns', [(40, 256), (700, 1024), (5000, 256), (5000, 2048)])
+@pytest.mark.parametrize('value', [float('inf'), float('nan')])
+def test_an_adapter_that_is_not_finite_stays_with_its_rows(rows, columns, value):
+    layout = U.Layout([rows], 1)
+    x, w, a, b, _ = _lora_inputs(layout, 3, 16, 512, columns, True)
+    idx = (torch.arange(rows) % 4 - 1).to(torch.int32)
+    want, size, low = _lora(x, w, a, b, None, idx, layout)
+    b[1, 0, 77, 3] = value
+    y = deep_ep.grouped_lora_linear(_dev(x), _dev(w[0]), _dev(a[:, 0]), _dev(b[:, 0]), _dev(idx))
+    more = (low * (2.0 ** -17 + 1024 * U.STEP_F32)).expand(size.shape)
+    hers = torch.zeros(size.shape, dtype=torch.bool)
+    hers[idx == 1, 77] = True
+    assert not torch.isfinite(y.cpu()[hers]).any()
+    U.assert_sum(y.cpu()[~hers], want[~hers], size[~hers], 512, more=more[~hers])
+    # the first matrix: a row's low-rank row is infinite or NaN, and all of its result
+    a[2, 0, 5, 100] = value
+    y = deep_ep.grouped_lora_linear(_dev(x), _dev(w[0]), _dev(a[:, 0]), _dev(b[:, 0]), _dev(idx)).cpu()
+    hers[idx == 2] = True
+    assert not torch.isfinite(y[hers]).any()
+    U.assert_sum(y[~hers], want[~hers], size[~hers], 512, more=more[~hers])
+
+
+def test_two_calls_at_once():
+    """On two streams, each with its workspaces."""
+    x, w = _dev(U.normal(1, 64, 7168)), [_dev(U.normal(2 + i, 512, 7168)) for i in range(2)]
+    a, b, idx = _dev(U.normal(4, 2, 16, 7168)), _dev(U.normal(5, 2, 512, 16)), (torch.arange(64, dtype=torch.int32) % 2).to(DEV)
+    want = [deep_ep.grouped_lora_linear(x, m, a, b, idx) for m in w]
+    grads = [deep_ep.grouped_linear_grad(want[0], x, m)[0] for m in w]
+    streams, got = [torch.cuda.Stream() for _ in w], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, m, g in zip(streams, w, got):
+            with torch.cuda.stream(s):
+                g.append((deep_ep.grouped_lora_linear(x, m, a, b, idx), deep_ep.grouped_linear_grad(want[0], x, m)[0]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y, g in got[i]:
+            assert torch.equal(y, want[i]) and torch.equal(g, grads[i])
+
+
 def test_adapters_as_views():
     """Matrices of adapters and experts inside larger tensors, and one that all adapters share."""
     layout = U.Layout([20, 3, 40], 8)

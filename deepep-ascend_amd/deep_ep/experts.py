@@ -147,7 +147,7 @@ def grouped_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Ten
         lora_a: `[adapters, experts, R, K]` bfloat16, lora_b: `[adapters, experts, N, R]`; without the experts' dimension where there is one.
             R is a multiple of 8 up to 64.
         adapter_idx: `[rows]` int32; a row whose number is outside `[0, adapters)` has no adapter.  `expand_token_index` makes it from
-            the tokens' numbers.
+            the tokens' numbers.  An adapter with infinities or NaN changes the rows that have it, no others.
         scales: `[adapters]` float32 or None.
         layout, out, do_zero_padding: as for `grouped_linear`.
 

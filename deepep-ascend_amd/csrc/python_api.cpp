@@ -795,7 +795,11 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
 void in_one_stream_if_captured() {
     const auto current = c10::hip::getCurrentHIPStream();
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();      // (the legacy stream beside another thread's capture: not captured itself)
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::get_current_node();
     for (const auto& edge : node->next_edges()) {
         if (!edge.is_valid() || dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;

@@ -5,14 +5,15 @@
 // contract and every launch lives behind the C ABI in libdeep_ep_hip.so.
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <memory>
+#include <numeric>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -598,18 +599,49 @@ void on_current_device(std::initializer_list<const at::Tensor*> tensors) {
 }
 const at::Tensor* of(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 
-// (the result, allocated where the caller brings none)
-// A result where an operand lies would be read again by other workgroups.
-void apart(const at::Tensor& out, std::initializer_list<const at::Tensor*> operands) {
-    for (const at::Tensor* t : operands) {
-        if (t == nullptr) continue;
-        const auto overlap = at::get_overlap_status(out, *t);
-        EP_PY_ASSERT(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial);
+// Where a tensor lies: runs of `run` bytes, their first bytes multiples of `step` apart (0: there is one run).
+struct Bytes {
+    uintptr_t first = 0, end = 0;
+    int64_t run = 0, step = 0;
+};
+Bytes bytes_of(const at::Tensor& t) {
+    Bytes b;
+    if (t.numel() == 0) return b;
+    c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;      // (bytes between entries, entries), innermost first
+    for (int i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) != 0) dims.emplace_back(t.stride(i) * (int64_t)t.element_size(), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    b.run = (int64_t)t.element_size();
+    int64_t last = 0;
+    for (const auto& [stride, size] : dims) {
+        last += stride * (size - 1);
+        if (b.step == 0 && stride == b.run) b.run *= size;
+        else b.step = std::gcd(b.step, stride);
     }
+    b.first = (uintptr_t)t.const_data_ptr();
+    b.end = b.first + last + t.element_size();
+    return b;
+}
+// Whether two tensors have no byte in common: one lies behind the other, or beside it, as columns of one matrix do.  (Of two that share none
+// in a less regular way this is not seen.)
+bool disjoint(const Bytes& a, const Bytes& b) {
+    if (a.end <= b.first || b.end <= a.first) return true;
+    const int64_t step = std::gcd(a.step, b.step);
+    if (step == 0) return false;
+    const int64_t apart = (int64_t)(b.first - a.first) % step, at = apart < 0 ? apart + step : apart;
+    return at >= a.run && at + b.run <= step;
+}
+// A result where an operand lies would be read again by other workgroups.
+void apart(const OptTensor& out, std::initializer_list<const at::Tensor*> operands) {
+    if (!out.has_value()) return;
+    const Bytes mine = bytes_of(*out);
+    for (const at::Tensor* t : operands)
+        if (t != nullptr && !disjoint(mine, bytes_of(*t))) throw EpPyError("a result must not lie on an operand");
 }
 
 at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf,
                        const OptTensor& psum, int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
+    apart(out, {&x, of(x_sf), &weight, of(weight_sf), of(psum)});
     on_current_device({&x, of(x_sf), &weight, of(weight_sf), of(psum), of(out)});
     EP_PY_ASSERT(x.dim() == 2);
     a.x = desc(x);
@@ -620,7 +652,6 @@ at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const O
         a.weight_sf = expert_matrix(*weight_sf, a.weight_sf_expert_stride);
     }
     a.psum_num_recv_tokens_per_expert = desc(psum);
-    if (out.has_value()) apart(*out, {&x, of(x_sf), &weight, of(weight_sf), of(psum)});
     const at::Tensor y = out.has_value() ? *out : alloc({x.size(0), weight.size(transpose_weight ? -1 : -2)}, at::kBFloat16, x.device());
     a.out = desc(y);
     a.num_experts = num_matrices(weight);
@@ -669,10 +700,10 @@ ep_tensor_t adapter_matrix(const at::Tensor& t, int num_adapters, int num_expert
 at::Tensor grouped_lora_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& lora_a, const at::Tensor& lora_b,
                                const at::Tensor& adapter_idx, const OptTensor& scales, const OptTensor& psum, int alignment, const OptTensor& out,
                                int zero_rows) {
-    on_current_device({&lora_a, &lora_b, &adapter_idx, of(scales)});
-    if (out.has_value()) apart(*out, {&lora_a, &lora_b, &adapter_idx, of(scales)});
+    apart(out, {&lora_a, &lora_b, &adapter_idx, of(scales)});
     ep_grouped_lora_args_t a{};
     const at::Tensor y = fill_linear(a.linear, x, std::nullopt, weight, std::nullopt, psum, alignment, out, zero_rows, false);
+    on_current_device({&lora_a, &lora_b, &adapter_idx, of(scales)});
     EP_PY_ASSERT(lora_a.dim() >= 3);
     a.num_adapters = (int)lora_a.size(0);
     a.lora_a = adapter_matrix(lora_a, a.num_adapters, a.linear.num_experts, a.lora_a_adapter_stride, a.lora_a_expert_stride);
@@ -701,9 +732,9 @@ at::Tensor expand_token_index(const at::Tensor& values, const at::Tensor& src_me
 
 at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, const OptTensor& psum, int num_experts, int alignment,
                                const OptTensor& out, bool accumulate) {
+    apart(out, {&grad, &x, of(psum)});
     on_current_device({&grad, &x, of(psum), of(out)});
     EP_PY_ASSERT(grad.dim() == 2 && x.dim() == 2);
-    if (out.has_value()) apart(*out, {&grad, &x, of(psum)});
     const at::Tensor w = out.has_value() ? *out : alloc({num_experts, grad.size(1), x.size(1)}, at::kBFloat16, x.device());
     ep_grouped_weight_grad_args_t a{};
     a.grad = desc(grad);
@@ -727,10 +758,10 @@ at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, cons
 
 std::tuple<at::Tensor, OptTensor> swiglu(const at::Tensor& h, const OptTensor& weights, const OptTensor& psum, int num_experts, int alignment,
                                          bool quantise, const OptTensor& out, const OptTensor& out_sf, int zero_rows) {
+    apart(out, {&h, of(weights), of(psum)});
+    apart(out_sf, {&h, of(weights), of(psum), of(out)});
     on_current_device({&h, of(weights), of(psum), of(out), of(out_sf)});
     EP_PY_ASSERT(h.dim() == 2);
-    if (out.has_value()) apart(*out, {&h, of(weights), of(psum)});
-    if (out_sf.has_value()) apart(*out_sf, {&h, of(weights), of(psum), of(out)});
     const int64_t rows = h.size(0), channels = h.size(1) / 2;
     const at::Tensor y = out.has_value() ? *out : alloc({rows, channels}, quantise ? at::kFloat8_e4m3fn : at::kBFloat16, h.device());
     OptTensor sf = out_sf;

@@ -19,7 +19,7 @@ The reference leaves the experts to its callers; these are entry points of this 
 * hold sums in 32 bits and round once; nothing is added atomically, results are the same from call to call.
 
 A backward pass can be recorded into a HIP graph too, but not while an eager graph of the same leaves lives (RuntimeError): end that one first, or
-record `grouped_linear_grad` and `swiglu_grad`.  `out` must not lie on an operand.
+record `grouped_linear_grad` and `swiglu_grad`.  `out` must not lie on an operand (an error); disjoint columns of one matrix may be both.
 
 Rows may have any stride that keeps them on 16 bytes; channels are contiguous, and come in multiples of 8 (16 for FP8).
 """

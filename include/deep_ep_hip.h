@@ -320,7 +320,8 @@ int ep_combine_begin_event(ep_buffer_t* buf, const ep_combine_args_t* args, void
  * Counts are read on the device only: nothing waits for the host, and rows that the counts place outside the tensors are
  * left out.  Rows of no expert (padding, and what lies behind the last expert's) take no part: they are read for
  * nothing and stay as they were in the results, or become zeros as zero_rows says.  Sums are held in 32 bits and rounded once.  Rows are addressed with their stride; channels are
- * contiguous, start on 16 bytes and come in multiples of 8 (BF16) or 16 (FP8 depth). */
+ * contiguous, start on 16 bytes and come in multiples of 8 (BF16) or 16 (FP8 depth).  No result may lie on an operand or on
+ * a workspace (not checked here). */
 /* zero_rows: which rows of no expert are written, as zeros */
 enum ep_zero_rows {
     EP_ZERO_NONE = 0,

@@ -1,0 +1,75 @@
+"""Calls of the experts' computation that the package refuses before anything touches a GPU."""
+import pytest
+import torch
+
+import deep_ep
+
+REFUSED = 'a result must not lie on an operand'
+ELSEWHERE = 'must live on the GPU'      # what a call of host tensors that nothing else is wrong with ends with
+
+
+def _bf16(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def _ends_with(message, call, *args, **kwargs):
+    with pytest.raises(deep_ep._C.EPException, match=message):
+        call(*args, **kwargs)
+
+
+# columns of x and of the result in one buffer of 8 x 256
+@pytest.mark.parametrize('x,out,message', [
+    ((0, 64), (0, 64), REFUSED), ((0, 64), (32, 96), REFUSED), ((32, 96), (0, 64), REFUSED), ((64, 128), (120, 184), REFUSED),
+    ((0, 64), (64, 128), ELSEWHERE), ((192, 256), (0, 64), ELSEWHERE), ((0, 64), (192, 256), ELSEWHERE)])
+def test_columns_of_one_matrix(x, out, message):
+    wide = _bf16(8, 256)
+    x, out = wide[:, slice(*x)], wide[:, slice(*out)]
+    _ends_with(message, deep_ep.grouped_linear, x, _bf16(64, 64), out=out)
+    _ends_with(message, deep_ep.grouped_linear, x[3:], _bf16(64, 64), out=out[:5])
+    idx = torch.zeros(8, dtype=torch.int32)
+    _ends_with(message, deep_ep.grouped_lora_linear, x, _bf16(64, 64), _bf16(1, 8, 64), _bf16(1, 64, 8), idx, out=out)
+    _ends_with(message, deep_ep.swiglu, x, out=out)      # (of other columns too: shapes are looked at behind this)
+
+
+def test_rows_of_one_matrix():
+    wide = _bf16(16, 64)
+    w = _bf16(64, 64)
+    _ends_with(REFUSED, deep_ep.grouped_linear, wide[:8], w, out=wide[7:15])
+    _ends_with(REFUSED, deep_ep.grouped_linear, wide[0::2], w, out=wide[0:8])
+    _ends_with(ELSEWHERE, deep_ep.grouped_linear, wide[:8], w, out=wide[8:])
+    _ends_with(ELSEWHERE, deep_ep.grouped_linear, wide[0::2], w, out=wide[1::2])
+    _ends_with(ELSEWHERE, deep_ep.grouped_linear, wide[:0], w, out=wide[:0])
+
+
+def test_every_operand_is_looked_at():
+    layout, idx = (torch.tensor([8, 16], dtype=torch.int32), 8), torch.zeros(16, dtype=torch.int32)
+    wide = _bf16(2, 16, 96)
+    x, out = _bf16(16, 64), wide[0, :, :16]
+    _ends_with(REFUSED, deep_ep.grouped_linear, x, wide[:, :, 8:72], layout, out=out)
+    _ends_with(ELSEWHERE, deep_ep.grouped_linear, x, wide[:, :, 16:80], layout, out=out)
+    _ends_with(REFUSED, deep_ep.grouped_linear, x, _bf16(2, 16, 64), (out.view(torch.int32)[:1].reshape(-1)[:2], 8), out=out)
+    a, b = _bf16(3, 2, 8, 96), _bf16(3, 2, 16, 24)
+    _ends_with(REFUSED, deep_ep.grouped_lora_linear, x, _bf16(2, 16, 64), a[..., :64], b[..., :8], idx, layout, out=a[0].view(16, 96)[:, 48:64])
+    _ends_with(REFUSED, deep_ep.grouped_lora_linear, x, _bf16(2, 16, 64), a[..., :64], b[..., :8], idx, layout, out=b[1, 1, :, :16])
+    _ends_with(ELSEWHERE, deep_ep.grouped_lora_linear, x, _bf16(2, 16, 64), a[..., :64], b[..., :8], idx, layout, out=b[1, 1, :, 8:])
+    # fp8 rows with their scales behind them, the results of swiglu side by side
+    packed = torch.zeros(16, 64 + 16, dtype=torch.uint8)
+    q, sf = packed[:, :64].view(torch.float8_e4m3fn), packed[:, 64:68].view(torch.float32)
+    w = (_bf16(16, 64).to(torch.float8_e4m3fn), torch.zeros(1, 1))
+    bytes_ = packed.view(torch.bfloat16)
+    _ends_with(REFUSED, deep_ep.grouped_linear, (q, sf), w, out=torch.as_strided(bytes_, (16, 16), (40, 1), 24))
+    _ends_with(ELSEWHERE, deep_ep.swiglu, _bf16(16, 128), fused_fp8_quant=True, out=(q, sf))
+    _ends_with(REFUSED, deep_ep.swiglu, _bf16(16, 128), fused_fp8_quant=True, out=(q, packed[:, 60:64].view(torch.float32)))
+    h = _bf16(16, 192)
+    weights = h.view(torch.float32)[:, 64:65].reshape(-1)
+    _ends_with(REFUSED, deep_ep.swiglu, h[:, :128], None, weights, out=h[:, 128:])      # (the weights are its first two columns)
+    _ends_with(ELSEWHERE, deep_ep.swiglu, h[:, :64], None, weights, out=h[:, 136:168])
+    shared = torch.zeros(64)
+    _ends_with(REFUSED, deep_ep.swiglu, _bf16(16, 16), None, shared[:16], out=shared.view(torch.bfloat16).view(16, 8))
+
+
+def test_gradients_of_weights_and_their_operands():
+    wide = _bf16(64, 256)
+    grad, x = wide[:, :64], wide[:, 64:128]
+    for at, message in ((0, REFUSED), (32, REFUSED), (120, REFUSED), (128, ELSEWHERE), (192, ELSEWHERE)):
+        _ends_with(message, deep_ep.grouped_linear_grad, grad, x, _bf16(64, 64), need_x=False, grad_weight=wide[:, at:at + 64])

@@ -1,0 +1,43 @@
+"""Calls of the experts' computation that its documentation allows or refuses: results beside their operands, paths of large calls, counts
+that are not the tensors', autograd."""
+import pytest
+import torch
+
+import deep_ep
+import experts_util as U
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def _dev(t):
+    return tuple(x.to(DEV) for x in t) if isinstance(t, tuple) else t.to(DEV)
+
+
+@pytest.mark.parametrize('rows', [20, 700])
+def test_results_beside_their_operands(rows):
+    """Columns of one matrix are operand and result."""
+    x, w = _dev(U.normal(1, rows, 256)), _dev(U.normal(2, 136, 256))
+    want = deep_ep.grouped_linear(x, w)
+    wide = torch.full((rows, 640), 77.0, dtype=torch.bfloat16, device=DEV)
+    vx, out = wide[:, 64:320].copy_(x), wide[:, 320:456]
+    assert torch.equal(deep_ep.grouped_linear(vx, w, out=out), want)
+    assert torch.equal(vx, x) and (wide[:, :64] == 77).all() and (wide[:, 456:] == 77).all()
+    activated = deep_ep.swiglu(x)
+    assert torch.equal(deep_ep.swiglu(vx, out=wide[:, 480:608]), activated)
+    grad = torch.zeros(rows, 136, dtype=torch.bfloat16, device=DEV).copy_(want)
+    _, gw = deep_ep.grouped_linear_grad(grad, x, w, need_x=False)
+    ww = torch.zeros(136, 512, dtype=torch.bfloat16, device=DEV)
+    vw = ww[:, :256].copy_(w)
+    _, vgw = deep_ep.grouped_linear_grad(out, vx, vw, need_x=False, grad_weight=ww[:, 256:])
+    assert torch.equal(vgw, gw) and torch.equal(vw, w)
+
+
+def test_results_on_columns_of_their_operands_are_refused():
+    wide, w = torch.zeros(300, 640, dtype=torch.bfloat16, device=DEV), _dev(U.normal(2, 256, 256))
+    for at in (0, 8, 248):
+        with pytest.raises(deep_ep._C.EPException, match='must not lie on an operand'):
+            deep_ep.grouped_linear(wide[:, :256], w, out=wide[:, at:at + 256])
+        with pytest.raises(deep_ep._C.EPException, match='must not lie on an operand'):
+            deep_ep.swiglu(wide[:, :256], out=wide[:, at:at + 128])
+    assert (wide == 0).all()

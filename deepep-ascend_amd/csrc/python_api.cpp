@@ -588,8 +588,10 @@ ep_tensor_t expert_matrix(const at::Tensor& t, int64_t& expert_stride) {
 }
 int num_matrices(const at::Tensor& t) { return t.dim() == 3 ? (int)t.size(0) : 1; }
 
-// Kernels run on the current device: everything they are given has to be there.
+// Kernels run on the current device: everything they are given has to be there.  A tangent would be lost with them.
 void on_current_device(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->_fw_grad(/*level=*/0).defined()) throw EpPyError("forward-mode gradients are not implemented");
     for (const at::Tensor* t : tensors)
         if (t != nullptr && !t->is_cuda()) throw EpPyError("every tensor handed to the EP kernels must live on the GPU");
     const int current = c10::hip::getCurrentHIPStream().device_index();

@@ -16,7 +16,8 @@ The reference leaves the experts to its callers; these are entry points of this 
   last expert's rows) are read for nothing.  They stay as they were in `out` and undefined in a result that is allocated here, but that
   `do_zero_padding` writes zeros into the padding rows, as a dispatch does;
 * are enqueued on the current stream, on the device of their tensors, which has to be the current one;
-* hold sums in 32 bits and round once; nothing is added atomically, results are the same from call to call.
+* hold sums in 32 bits and round once; nothing is added atomically, results are the same from call to call;
+* refuse tensors with a forward-mode tangent.
 
 A backward pass can be recorded into a HIP graph too, but not while an eager graph of the same leaves lives (RuntimeError): end that one first, or
 record `grouped_linear_grad` and `swiglu_grad`.  `out` must not lie on an operand (an error); disjoint columns of one matrix may be both.

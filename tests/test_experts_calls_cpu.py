@@ -73,3 +73,30 @@ def test_gradients_of_weights_and_their_operands():
     grad, x = wide[:, :64], wide[:, 64:128]
     for at, message in ((0, REFUSED), (32, REFUSED), (120, REFUSED), (128, ELSEWHERE), (192, ELSEWHERE)):
         _ends_with(message, deep_ep.grouped_linear_grad, grad, x, _bf16(64, 64), need_x=False, grad_weight=wide[:, at:at + 64])
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+    layout, idx = (torch.tensor([4], dtype=torch.int32), 1), torch.zeros(4, dtype=torch.int32)
+    x, w, a, b, scales = _bf16(4, 64), _bf16(1, 64, 64), _bf16(1, 1, 8, 64), _bf16(1, 1, 64, 8), torch.ones(1)
+    grad, q, qw = _bf16(4, 64), (_bf16(4, 64).to(torch.float8_e4m3fn), torch.ones(4, 1)), (_bf16(1, 64, 64).to(torch.float8_e4m3fn), torch.ones(1, 1, 1))
+    message = 'forward-mode gradients are not implemented'
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        _ends_with(message, deep_ep.grouped_linear, dual(x), w, layout)
+        _ends_with(message, deep_ep.grouped_linear, x, dual(w), layout)
+        _ends_with(message, deep_ep.grouped_linear, dual(x.detach().requires_grad_()), w, layout)
+        _ends_with(message, deep_ep.grouped_linear, (q[0], dual(q[1])), qw, layout)
+        _ends_with(message, deep_ep.grouped_linear, q, (qw[0], dual(qw[1])), layout)
+        _ends_with(message, deep_ep.grouped_linear_grad, dual(grad), x, w, layout)
+        _ends_with(message, deep_ep.grouped_linear_grad, grad, x, dual(w), layout, need_weight=False)
+        _ends_with(message, deep_ep.grouped_linear_grad, grad, dual(x), w, layout, need_x=False)
+        _ends_with(message, deep_ep.swiglu, dual(x), layout)
+        _ends_with(message, deep_ep.swiglu, x, layout, dual(torch.ones(4)))
+        _ends_with(message, deep_ep.swiglu_grad, grad[:, :32], dual(x), layout)
+        _ends_with(message, deep_ep.swiglu_grad, grad[:, :32], x, layout, dual(torch.ones(4)))
+        _ends_with(message, deep_ep.grouped_lora_linear, dual(x), w, a, b, idx, layout)
+        _ends_with(ELSEWHERE, deep_ep.grouped_linear, x, w, layout)
+    with torch.no_grad(), forward_ad.dual_level():
+        _ends_with(message, deep_ep.grouped_linear, forward_ad.make_dual(x, x), w, layout)

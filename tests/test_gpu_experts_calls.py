@@ -41,3 +41,15 @@ def test_results_on_columns_of_their_operands_are_refused():
         with pytest.raises(deep_ep._C.EPException, match='must not lie on an operand'):
             deep_ep.swiglu(wide[:, :256], out=wide[:, at:at + 128])
     assert (wide == 0).all()
+
+
+def test_forward_mode_tangents_of_adapters_are_refused():
+    from torch.autograd import forward_ad
+    x, w, a, b, scales = (_dev(U.normal(i, *shape)) for i, shape in enumerate([(4, 64), (64, 64), (1, 8, 64), (1, 64, 8), (1,)]))
+    idx, scales = torch.zeros(4, dtype=torch.int32, device=DEV), scales.float()
+    with forward_ad.dual_level():
+        for i in range(3):
+            tensors = [a, b, scales]
+            tensors[i] = forward_ad.make_dual(tensors[i], torch.ones_like(tensors[i]))
+            with pytest.raises(deep_ep._C.EPException, match='forward-mode gradients are not implemented'):
+                deep_ep.grouped_lora_linear(x, w, *tensors[:2], idx, scales=tensors[2])

@@ -641,6 +641,11 @@ void apart(const OptTensor& out, std::initializer_list<const at::Tensor*> operan
         if (t != nullptr && !disjoint(mine, bytes_of(*t))) throw EpPyError("a result must not lie on an operand");
 }
 
+// A graph that saved the tensor notices what a call stored into it.  (Inference tensors have no version.)
+void stored(const OptTensor& out) {
+    if (out.has_value() && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor fill_linear(ep_grouped_linear_args_t& a, const at::Tensor& x, const OptTensor& x_sf, const at::Tensor& weight, const OptTensor& weight_sf,
                        const OptTensor& psum, int alignment, const OptTensor& out, int zero_rows, bool transpose_weight) {
     apart(out, {&x, of(x_sf), &weight, of(weight_sf), of(psum)});
@@ -679,6 +684,7 @@ at::Tensor grouped_linear(const at::Tensor& x, const OptTensor& x_sf, const at::
     const at::Tensor y = fill_linear(a, x, x_sf, weight, weight_sf, psum, alignment, out, zero_rows, transpose_weight);
     const at::Tensor workspace = linear_workspace(a, x.device(), false);
     check(ep_grouped_linear(&a));
+    stored(out);
     return y;
 }
 
@@ -720,6 +726,7 @@ at::Tensor grouped_lora_linear(const at::Tensor& x, const at::Tensor& weight, co
     }
     const at::Tensor of_linear = linear_workspace(a.linear, x.device(), true);
     check(ep_grouped_lora_linear(&a));
+    stored(out);
     return y;
 }
 
@@ -755,6 +762,7 @@ at::Tensor grouped_weight_grad(const at::Tensor& grad, const at::Tensor& x, cons
     }
     a.stream = current_stream();
     check(ep_grouped_weight_grad(&a));
+    stored(out);
     return w;
 }
 
@@ -780,6 +788,8 @@ std::tuple<at::Tensor, OptTensor> swiglu(const at::Tensor& h, const OptTensor& w
     a.zero_rows = zero_rows;
     a.stream = current_stream();
     check(ep_swiglu(&a));
+    stored(out);
+    stored(out_sf);
     return {y, sf};
 }
 

@@ -53,3 +53,43 @@ def test_forward_mode_tangents_of_adapters_are_refused():
             tensors[i] = forward_ad.make_dual(tensors[i], torch.ones_like(tensors[i]))
             with pytest.raises(deep_ep._C.EPException, match='forward-mode gradients are not implemented'):
                 deep_ep.grouped_lora_linear(x, w, *tensors[:2], idx, scales=tensors[2])
+
+
+def _stale(saved, store):
+    """A graph that saved `saved` notices what `store` wrote into it."""
+    w = _dev(U.normal(9, 16, saved.size(1))).requires_grad_()
+    y = deep_ep.grouped_linear(saved, w)
+    before = saved._version
+    store()
+    assert saved._version > before
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
+def test_stored_results_are_noticed_by_graphs_that_saved_the_tensor():
+    x, w, a, b = (_dev(U.normal(i, *shape)) for i, shape in enumerate([(8, 64), (64, 64), (1, 8, 64), (1, 64, 8)]))
+    idx, h, grad = torch.zeros(8, dtype=torch.int32, device=DEV), _dev(U.normal(5, 8, 128)), _dev(U.normal(6, 8, 8))
+    out = torch.zeros(8, 64, dtype=torch.bfloat16, device=DEV)
+    _stale(out, lambda: deep_ep.grouped_linear(x, w, out=out))
+    _stale(out, lambda: deep_ep.grouped_lora_linear(x, w, a, b, idx, out=out))
+    _stale(out, lambda: deep_ep.swiglu(h, out=out))
+    wide = torch.zeros(8, 128, dtype=torch.bfloat16, device=DEV)
+    _stale(wide, lambda: deep_ep.grouped_linear(x, w, out=wide[:, 64:]))           # (a view has its base's version)
+    _stale(out, lambda: deep_ep.grouped_linear_grad(grad, x, out, need_x=False, grad_weight=out))
+    q, sf = torch.zeros(8, 64, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn), torch.zeros(8, 1, device=DEV)
+    versions = q._version, sf._version
+    deep_ep.swiglu(h, fused_fp8_quant=True, out=(q, sf))
+    assert q._version > versions[0] and sf._version > versions[1]
+    # what only lies beside the result, or is only read, keeps its version
+    versions = x._version, w._version, h._version
+    deep_ep.swiglu(h, out=deep_ep.grouped_linear(x, w, out=out))
+    assert versions == (x._version, w._version, h._version)
+
+
+def test_results_in_inference_mode():
+    x, w = _dev(U.normal(1, 8, 64)), _dev(U.normal(2, 64, 64))
+    want = deep_ep.grouped_linear(x, w)
+    with torch.inference_mode():
+        out = torch.zeros_like(want)
+        assert torch.equal(deep_ep.grouped_linear(x, w, out=out), want)
+    assert torch.equal(deep_ep.grouped_linear(x, w, out=out), want)      # (such a tensor has no version)

@@ -20,7 +20,8 @@ The reference leaves the experts to its callers; these are entry points of this 
 * refuse tensors with a forward-mode tangent.
 
 A backward pass can be recorded into a HIP graph too, but not while an eager graph of the same leaves lives (RuntimeError): end that one first, or
-record `grouped_linear_grad` and `swiglu_grad`.  `out` must not lie on an operand (an error); disjoint columns of one matrix may be both.
+record `grouped_linear_grad` and `swiglu_grad`.  `out` must not lie on an operand (an error; disjoint columns of one matrix may be both),
+nor ask for a gradient itself.
 
 Rows may have any stride that keeps them on 16 bytes; channels are contiguous, and come in multiples of 8 (16 for FP8).
 """
@@ -70,7 +71,7 @@ def grouped_linear(x: _TensorOrPair, weight: _TensorOrPair, layout: _Layout = No
     is zero, whatever the result's gradient holds there.
     """
     (x, x_sf), (weight, weight_sf), (psum, alignment) = _pair(x), _pair(weight), _layout(layout)
-    if _wants_grad(x, weight, x_sf, weight_sf):
+    if _wants_grad(x, weight, x_sf, weight_sf, out):
         if out is not None or x_sf is not None or weight_sf is not None:
             raise AssertionError('gradients are implemented for bfloat16 and without `out`')
         return _native.grouped_linear_autograd(x, weight, psum, alignment, do_zero_padding)
@@ -97,6 +98,8 @@ def grouped_linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
         assert not accumulate, 'accumulate=True adds to `grad_weight`'
         grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
     assert grad_weight.shape == weight.shape
+    if _wants_grad(grad_weight):
+        raise AssertionError('gradients are stored into tensors without a gradient of their own')
     return grad_x, _native.grouped_weight_grad(grad, x, psum, weight.size(0) if weight.dim() == 3 else 1, alignment, grad_weight, accumulate)
 
 
@@ -121,7 +124,7 @@ def swiglu(h: torch.Tensor, layout: _Layout = None, topk_weights: Optional[torch
     psum, alignment = _layout(layout)
     out, out_sf = _pair(out)
     assert out is None or (out_sf is not None) == fused_fp8_quant, 'a pair of tensors is what a quantised result is stored into'
-    if _wants_grad(h, topk_weights):
+    if _wants_grad(h, topk_weights, out, out_sf):
         if out is not None or fused_fp8_quant:
             raise AssertionError('gradients are implemented for bfloat16 and without `out`')
         return _native.swiglu_autograd(h, topk_weights, psum, _num_experts(psum), alignment, do_zero_padding)
@@ -155,7 +158,7 @@ def grouped_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Ten
     The low-rank rows are held in 32 bits.  For inference: no gradients.
     """
     psum, alignment = _layout(layout)
-    if _wants_grad(x, weight, lora_a, lora_b, scales):
+    if _wants_grad(x, weight, lora_a, lora_b, scales, out):
         raise AssertionError('gradients of adapters are not implemented')
     return _native.grouped_lora_linear(x, weight, lora_a, lora_b, adapter_idx, scales, psum, alignment, out, do_zero_padding)
 

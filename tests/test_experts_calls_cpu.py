@@ -100,3 +100,20 @@ def test_forward_mode_tangents_are_refused():
         _ends_with(ELSEWHERE, deep_ep.grouped_linear, x, w, layout)
     with torch.no_grad(), forward_ad.dual_level():
         _ends_with(message, deep_ep.grouped_linear, forward_ad.make_dual(x, x), w, layout)
+
+
+def test_results_with_a_gradient_of_their_own_are_refused():
+    """Such a tensor's graph would not know of the value that is stored into it."""
+    x, w, h = _bf16(4, 64), _bf16(64, 64), _bf16(4, 128)
+    a, b, idx = _bf16(1, 8, 64), _bf16(1, 64, 8), torch.zeros(4, dtype=torch.int32)
+    leaf = _bf16(4, 64).requires_grad_()
+    for out in (leaf, leaf * 2):
+        for call, *args in ((deep_ep.grouped_linear, x, w), (deep_ep.swiglu, h), (deep_ep.grouped_lora_linear, x, w, a, b, idx)):
+            with pytest.raises(AssertionError, match='gradients'):
+                call(*args, out=out)
+            with torch.no_grad():
+                _ends_with(ELSEWHERE, call, *args, out=out)
+        with pytest.raises(AssertionError, match='gradients'):
+            deep_ep.grouped_linear_grad(x, x, _bf16(4, 64), need_x=False, grad_weight=out)
+    with pytest.raises(AssertionError, match='gradients'):
+        deep_ep.swiglu(h, fused_fp8_quant=True, out=(_bf16(4, 64).to(torch.float8_e4m3fn), torch.zeros(4, 1, requires_grad=True)))

@@ -52,6 +52,11 @@ bool row_major(const ep_tensor_t& t) {
     if (t.size[0] > 1 and (t.stride[0] < t.size[1] or t.stride[0] * elem % 16 != 0)) return false;
     return ((uintptr_t)t.data & 15) == 0;
 }
+// Every value of a matrix has a place of its own.
+bool apart(const ep_tensor_t& t) {
+    const int inner = t.size[0] > 1 and (t.size[1] <= 1 or t.stride[0] < t.stride[1]) ? 0 : 1, outer = 1 - inner;
+    return (t.size[inner] <= 1 or t.stride[inner] > 0) and (t.size[outer] <= 1 or t.stride[outer] >= t.size[inner] * t.stride[inner]);
+}
 int64_t row_stride(const ep_tensor_t& t) { return t.size[0] > 1 ? t.stride[0] : (t.size[1] + 15) / 16 * 16; }
 
 // Bytes of a tile's rows are counted in 31 bits.
@@ -472,6 +477,7 @@ int ep_swiglu(const ep_swiglu_args_t* args) {
         EP_HOST_ASSERT(fp8 == present(sf));
         if (fp8) {
             EP_HOST_ASSERT(sf.ndim == 2 and sf.dtype == EP_DTYPE_F32 and sf.size[0] == out.size[0] and sf.size[1] == ceil_div(s.channels, 128));
+            EP_HOST_ASSERT(apart(sf));
             s.sf = (float*)sf.data;
             s.sf_row = sf.stride[0];
             s.sf_col = sf.stride[1];

@@ -393,7 +393,7 @@ typedef struct ep_swiglu_args {
     ep_tensor_t weights;                /* [M] fp32 (optional): gate weight of the row */
     ep_tensor_t psum_num_recv_tokens_per_expert;
     ep_tensor_t out;                    /* [M,I] BF16, or e4m3fn with out_sf */
-    ep_tensor_t out_sf;                 /* [M, ceil(I/128)] fp32, any strides */
+    ep_tensor_t out_sf;                 /* [M, ceil(I/128)] fp32, strides that keep them apart */
     int32_t num_experts, expert_alignment, zero_rows;
     void* stream;
 } ep_swiglu_args_t;

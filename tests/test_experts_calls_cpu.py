@@ -117,3 +117,25 @@ def test_results_with_a_gradient_of_their_own_are_refused():
             deep_ep.grouped_linear_grad(x, x, _bf16(4, 64), need_x=False, grad_weight=out)
     with pytest.raises(AssertionError, match='gradients'):
         deep_ep.swiglu(h, fused_fp8_quant=True, out=(_bf16(4, 64).to(torch.float8_e4m3fn), torch.zeros(4, 1, requires_grad=True)))
+
+
+@pytest.mark.parametrize('stride,ok', [((0, 1), False), ((0, 0), False), ((1, 0), False), ((1, 63), False), ((1, 1), False), ((-2, 1), False),
+                                       ((2, 1), True), ((1, 64), True), ((1, 80), True), ((5, 2), True)])
+def test_scales_that_lie_on_each_other_are_refused(stride, ok):
+    """Scales that swiglu stores, [64, 2]: every one has a place of its own."""
+    import ctypes
+    import test_experts_cpu as C
+    lib = deep_ep._C._lib
+    a = C.Swiglu()
+    sf = C.matrix(64, 2, C.F32)
+    sf.stride[0], sf.stride[1] = stride
+    for k, v in dict(h=C.matrix(64, 512), psum=C.vector(4, C.I32), out=C.matrix(64, 256, C.FP8), out_sf=sf, num_experts=4, expert_alignment=16).items():
+        setattr(a, k, v)
+    lib.ep_swiglu.argtypes = [ctypes.c_void_p]
+    if torch.cuda.is_available() and ok:
+        pytest.skip('the addresses are not memory')
+    assert lib.ep_swiglu(ctypes.addressof(a)) != 0
+    lib.ep_last_error.restype = ctypes.c_char_p
+    message = lib.ep_last_error().decode()
+    # (what is right comes as far as the missing GPU)
+    assert message.startswith('Assertion exception (ep_experts.cpp:') != ok, message

@@ -16,6 +16,7 @@
 #include <numeric>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/deep_ep_hip.h"
@@ -834,7 +835,8 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
 }
 
 // A captured pass whose leaves an eager graph, still alive, has tied to another stream would bring that stream into the capture, which
-// breaks the capture and, with it, the process: an error in time.
+// breaks the capture and, with it, the process: an error in time.  The leaves may lie behind other nodes (weights that are cast); those that the
+// pass does not go to do not count.
 void in_one_stream_if_captured() {
     const auto current = c10::hip::getCurrentHIPStream();
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -843,13 +845,20 @@ void in_one_stream_if_captured() {
         return;
     }
     if (status == hipStreamCaptureStatusNone) return;
-    const auto node = torch::autograd::get_current_node();
-    for (const auto& edge : node->next_edges()) {
-        if (!edge.is_valid() || dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
-        const auto stream = edge.function->stream();
-        if (stream.has_value() && stream->id() != current.id())
-            throw std::runtime_error("a backward pass is captured into a graph while an eager one of the same leaves lives: end that one first, or capture "
-                                     "grouped_linear_grad and swiglu_grad");
+    std::vector<torch::autograd::Node*> ahead{torch::autograd::get_current_node().get()};
+    std::unordered_set<torch::autograd::Node*> seen(ahead.begin(), ahead.end());
+    while (!ahead.empty()) {
+        torch::autograd::Node* const node = ahead.back();
+        ahead.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) != nullptr) {
+            const auto stream = node->stream();
+            if (stream.has_value() && stream->id() != current.id())
+                throw std::runtime_error("a backward pass is captured into a graph while an eager one of the same leaves lives: end that one first, or "
+                                         "capture grouped_linear_grad and swiglu_grad");
+        }
+        for (size_t i = 0; i < node->num_outputs(); ++i)
+            if (node->task_should_compute_output(i) && seen.insert(node->next_edge(i).function.get()).second)
+                ahead.push_back(node->next_edge(i).function.get());
     }
 }
 

@@ -93,3 +93,51 @@ def test_results_in_inference_mode():
         out = torch.zeros_like(want)
         assert torch.equal(deep_ep.grouped_linear(x, w, out=out), want)
     assert torch.equal(deep_ep.grouped_linear(x, w, out=out), want)      # (such a tensor has no version)
+
+
+def _captured_while_alive(leaf, run):
+    """(the eager result, the error of a captured backward pass beside it, the graph)"""
+    eager = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run()
+        with pytest.raises(RuntimeError, match='while an eager one of the same leaves lives'):
+            y.backward(torch.ones_like(y))
+    graph.replay()
+    assert leaf.grad is None and torch.equal(y.detach(), eager.detach())
+    eager.backward(torch.ones_like(eager))
+    return leaf.grad
+
+
+def test_leaves_behind_other_nodes_are_seen_when_a_backward_pass_is_captured():
+    x, w = _dev(U.normal(1, 8, 64)), _dev(U.normal(2, 64, 64))
+    ones = torch.ones(8, 64, dtype=torch.bfloat16, device=DEV)
+    gx, gw = deep_ep.grouped_linear_grad(ones, x, w)
+    master = w.float().requires_grad_()
+    assert torch.equal(_captured_while_alive(master, lambda: deep_ep.grouped_linear(x, master.to(torch.bfloat16))), gw.float())
+    rows = x.float().requires_grad_()
+    assert torch.equal(_captured_while_alive(rows, lambda: deep_ep.grouped_linear(rows.view(64, 8).view(8, 64).to(torch.bfloat16), w)), gx.float())
+    gates = x.float().requires_grad_()
+    gh, _ = deep_ep.swiglu_grad(ones[:, :32].contiguous(), x)
+    assert torch.equal(_captured_while_alive(gates, lambda: deep_ep.swiglu(gates.to(torch.bfloat16))), gh.float())
+
+
+def test_leaves_that_a_captured_pass_does_not_go_to_may_be_an_eager_graphs():
+    x, w = _dev(U.normal(1, 8, 64)), _dev(U.normal(2, 64, 64)).requires_grad_()
+    grad = _dev(U.normal(3, 8, 64))
+    eager = deep_ep.grouped_linear(x, w)
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        y = deep_ep.grouped_linear(leaf, w)
+        return torch.autograd.grad(y, leaf, grad)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        x.copy_(U.normal(10 + seed, 8, 64)), grad.copy_(U.normal(20 + seed, 8, 64))
+        graph.replay()
+        got = captured.clone()
+        assert torch.equal(got, deep_ep.grouped_linear_grad(grad, x, w.detach(), need_weight=False)[0])
+        torch.cuda.synchronize()
+    assert eager.requires_grad

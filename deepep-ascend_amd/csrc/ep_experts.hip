@@ -335,10 +335,10 @@ __device__ __forceinline__ void low_ranks(const EpGemmArgs& a, int64_t row, int 
 // to 2048: 508 us, 6.1 TB/s).
 // Many rows: the matrix units' behind their operands.  A step of 256 x 256 is 64 KB from the L2 and 64 BF16 (32 FP8) matrix instructions a wave.
 // BF16 has room for two stages of the rows and three of the columns in LDS: 16384 rows, 8192 x 8192 weights run at 1320 TFLOP/s with two of both
-// and at 1400 with the third; the matrix units are busy 66 % of the time then, at the 1.95 GHz that power leaves them.
+// and at 1400 with the third; the matrix units are busy 72 % of the time then, at the clock that power leaves them.
 // FP8: a step is a group of channels, summed by itself in 32 bits and scaled with the row's and the block's scale as it is added (3 % of the time).
-// Its scales take what a third stage would need: 98304 rows, 7168 channels to 4096, at 1700 TFLOP/s, the matrix units busy 47 % of the time and
-// the waves waiting for a stage 29 %.  Fetching the step after that into the L2 made it slower, matrix instructions of 32 x 32 were level.
+// Its scales take 4 KB of the LDS, which a third stage of the columns would need to the last byte: 98304 rows, 7168 channels to 4096, at 1700 TFLOP/s, the matrix units busy 46 % of the time and
+// the waves waiting for a stage 27 %.  Fetching the step after that into the L2 made it slower, matrix instructions of 32 x 32 were level.
 template <int TM, int TN, int WR, int WC, int SR, int SC, bool FP8, bool COLUMNS_T, bool ROWS_T, bool OUT32, bool LORA = false,
           bool LOW_RANK = false>
 struct Gemm {

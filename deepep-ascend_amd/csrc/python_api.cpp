@@ -567,7 +567,7 @@ private:
     bool exact_sync_sizes_ = false;
 };
 
-// ---- the experts' computation (deep_ep/experts.py checks what the C ABI does not see: devices, overlapping kinds of arguments) ----
+// ---- the experts' computation: checked here is what the C ABI does not see (devices, results on operands, tangents) ----
 
 // Matrices of the experts, [E, N, K], or one matrix: what the C ABI takes of expert 0, and the stride between experts.
 ep_tensor_t expert_matrix(const at::Tensor& t, int64_t& expert_stride) {

@@ -16,7 +16,9 @@ The reference leaves the experts to its callers; these are entry points of this 
   last expert's rows) are read for nothing.  They stay as they were in `out` and undefined in a result that is allocated here, but that
   `do_zero_padding` writes zeros into the padding rows, as a dispatch does;
 * are enqueued on the current stream, on the device of their tensors, which has to be the current one;
-* hold sums in 32 bits and round once; nothing is added atomically, results are the same from call to call;
+* hold sums in 32 bits and round once; nothing is added atomically, results are the same from call to call.  Two places keep less: of eight
+  neighbouring channels' products of FP8 the matrix instruction leaves out what is below 2^-13 of the largest (about 3e-5 of a result, beside
+  the 2^-8 of its rounding), and `grouped_lora_linear` may keep 2^-17 of a low-rank row;
 * refuse tensors with a forward-mode tangent.
 
 A backward pass can be recorded into a HIP graph too, but not while an eager graph of the same leaves lives (RuntimeError): end that one first, or
@@ -155,7 +157,8 @@ def grouped_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Ten
         scales: `[adapters]` float32 or None.
         layout, out, do_zero_padding: as for `grouped_linear`.
 
-    The low-rank rows are held in 32 bits.  For inference: no gradients.
+    The low-rank rows are sums in 32 bits.  Where a tile of rows has few adapters they go on as two bfloat16 (2^-17 of them is kept), elsewhere in
+    32 bits: a row's last bits can depend on the other rows of the call.  For inference: no gradients.
     """
     psum, alignment = _layout(layout)
     if _wants_grad(x, weight, lora_a, lora_b, scales, out):

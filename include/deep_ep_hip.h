@@ -319,7 +319,9 @@ int ep_combine_begin_event(ep_buffer_t* buf, const ep_combine_args_t* args, void
  * say which rows are an expert's (from align(psum[e - 1]) up to psum[e]); without a psum (absent) one expert has all rows.
  * Counts are read on the device only: nothing waits for the host, and rows that the counts place outside the tensors are
  * left out.  Rows of no expert (padding, and what lies behind the last expert's) take no part: they are read for
- * nothing and stay as they were in the results, or become zeros as zero_rows says.  Sums are held in 32 bits and rounded once.  Rows are addressed with their stride; channels are
+ * nothing and stay as they were in the results, or become zeros as zero_rows says.  Sums are held in 32 bits and rounded once; of
+ * eight neighbouring channels' FP8 products the matrix instruction leaves out what is below 2^-13 of the largest.  Rows are
+ * addressed with their stride; channels are
  * contiguous, start on 16 bytes and come in multiples of 8 (BF16) or 16 (FP8 depth).  No result may lie on an operand or on
  * a workspace (not checked here). */
 /* zero_rows: which rows of no expert are written, as zeros */
@@ -349,7 +351,8 @@ int64_t ep_grouped_linear_workspace_bytes(int64_t num_rows, int num_experts, int
 int ep_grouped_linear(const ep_grouped_linear_args_t* args);
 
 /* Low-rank adapters of many requests beside the product: out[m] = W[e(m)] x[m] + scales[a] B[a,e(m)] (A[a,e(m)] x[m]) with
- * a = adapter_idx[m]; a row whose number is outside [0, num_adapters) has none.  BF16; the low-rank rows are held in 32 bits. */
+ * a = adapter_idx[m]; a row whose number is outside [0, num_adapters) has none.  BF16; the low-rank rows are sums in 32 bits, which go
+ * on as two BF16 (2^-17 of them) where a tile of rows has few adapters, in 32 bits elsewhere. */
 typedef struct ep_grouped_lora_args {
     ep_grouped_linear_args_t linear;
     ep_tensor_t lora_a;                 /* [R,K] BF16 of adapter 0 and expert 0, R a multiple of 8 up to EP_LORA_MAX_RANK */

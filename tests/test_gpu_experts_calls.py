@@ -317,3 +317,62 @@ def test_experts_of_several_partitions(R, max_tokens, E, K, A, sync):
         assert (got - want).norm() <= 3 * U.HALF_BF16 * want.norm()
     for buf in bufs:
         buf.destroy()
+
+
+# ---- rows and experts that are not finite ----------------------------------------------------------------------
+
+@pytest.mark.parametrize('counts', [[20, 3, 9], [300, 70, 513]])
+@pytest.mark.parametrize('depth', [256, 7168])
+@pytest.mark.parametrize('kind', ['bf16', 'fp8', 'lora', 'rows'])
+@pytest.mark.parametrize('value', [float('inf'), float('nan')])
+def test_what_is_not_finite_stays_with_its_row_and_expert(counts, depth, kind, value):
+    """A row's values do not reach another row, an expert's weights no other expert's rows: to the last bit what comes without them."""
+    layout = U.Layout(counts, 8)
+    x, w = U.normal(1, layout.rows, depth), U.normal(2, 3, 256, depth, scale=depth ** -0.5)
+    a, b = _dev(U.normal(3, 4, 3, 16, depth, scale=depth ** -0.5)), _dev(U.normal(4, 4, 3, 256, 16))
+    # (one adapter a tile, or none: rows beside one that is not finite are summed in the same order)
+    idx = torch.zeros(layout.rows, dtype=torch.int32, device=DEV)
+    psum = layout.on(DEV)
+
+    def run(x, w):
+        if kind == 'lora':
+            return deep_ep.grouped_lora_linear(_dev(x), _dev(w), a, b, idx, psum, do_zero_padding=True)
+        if kind == 'rows':
+            return deep_ep.grouped_linear_grad(_dev(x), _dev(x), _dev(w.transpose(1, 2).contiguous()), psum, need_weight=False, do_zero_padding=True)[0]
+        if kind == 'fp8':
+            q, sf = U.quantise_rows(torch.nan_to_num(x, 1.0, 1.0, 1.0))
+            sf[~torch.isfinite(x).all(dim=1)] = value
+            wq, wsf = U.quantise_weights(torch.nan_to_num(w, 1.0, 1.0, 1.0))
+            wsf[~torch.isfinite(w).all(dim=2).all(dim=1)] = value
+            return deep_ep.grouped_linear((_dev(q), _dev(sf)), (_dev(wq), _dev(wsf)), psum, do_zero_padding=True)
+        return deep_ep.grouped_linear(_dev(x), _dev(w), psum, do_zero_padding=True)
+    want = run(x, w)
+    bad = x.clone()
+    mine = torch.zeros(layout.rows, dtype=torch.bool)
+    for row in (0, layout.start[2] + counts[2] - 1):
+        bad[row, 5], mine[row] = value, True
+    got = run(bad, w)
+    assert not torch.isfinite(got[mine.to(DEV)]).any()
+    if kind == 'lora':      # (beside it, rows may take their low-rank rows in 32 bits instead of two BF16)
+        error = (got.double() - want.double())[~mine.to(DEV)].abs()
+        low = (_dev(x).double().abs() @ a[0].double().abs().amax(dim=0).t()) @ b[0].double().abs().amax(dim=0).t()
+        assert (error <= want[~mine.to(DEV)].double().abs() * 2 * U.HALF_BF16 + 2 * low[~mine.to(DEV)] * (2.0 ** -17 + depth * U.STEP_F32)).all()
+    else:
+        assert torch.equal(got[~mine.to(DEV)], want[~mine.to(DEV)])
+    bad, mine = w.clone(), torch.zeros(layout.rows, dtype=torch.bool)
+    bad[1, :, 5], mine[layout.slices()[1]] = value, True
+    got = run(x, bad)
+    assert not torch.isfinite(got[mine.to(DEV)]).any() and torch.equal(got[~mine.to(DEV)], want[~mine.to(DEV)])
+
+
+@pytest.mark.parametrize('value', [float('inf'), float('nan')])
+def test_gradients_of_what_is_not_finite_stay_with_their_expert(value):
+    layout = U.Layout([70, 40, 300], 8)
+    grad, x, w = U.normal(1, layout.rows, 136), U.normal(2, layout.rows, 264), _dev(U.normal(3, 3, 136, 264))
+    want = deep_ep.grouped_linear_grad(_dev(grad), _dev(x), w, layout.on(DEV), need_x=False)[1]
+    grad[layout.start[1] + 39, 7] = value
+    got = deep_ep.grouped_linear_grad(_dev(grad), _dev(x), w, layout.on(DEV), need_x=False)[1]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    assert not torch.isfinite(got[1, 7]).any()
+    rest = torch.arange(136) != 7
+    assert torch.equal(got[1, rest.to(DEV)], want[1, rest.to(DEV)])
